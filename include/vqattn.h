@@ -502,6 +502,72 @@ int vqa_count_step_f16(const void* q, const void* rope_cos, const void* rope_sin
                        const void* codebook, int32_t* cnt, float* vsum, void* out, float* lse, int B, int H, int C,
                        int D, const int64_t* strides, float sm_scale, vqa_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Paged key / value cache: pools of pages [n_pages, H, page, D] (page a power of two, 16 .. 4096), a block table
+ * [S, width] int32 that names the pages of every sequence in order, and per sequence its number of keys kv_lens [S] int32,
+ * new ones included.  The new rows of all sequences are packed back to back: those of sequence s are rows
+ * cu_q[s] .. cu_q[s + 1] (cu_q [S + 1] int32, not decreasing), and stand at positions kv_lens[s] - n .. kv_lens[s] - 1.
+ * Rows behind the last sequence are left alone.  A table entry outside [0, n_pages) is a page that is not there: nothing
+ * is written to it, it reads as zeros, its keys are hidden.  All of these are read on the device when the kernels run, and
+ * brought into range there: a recorded call can be replayed on new lengths and tables.
+ *
+ * Storage (e4m3 = 0): the element type.  e4m3 = 1: one byte per element plus one byte per row, value =
+ * e4m3 * 2^(byte - 127); the byte names the smallest power of two that brings the row into +-448.  Pages [.., page, D]
+ * bytes, exponents k_exp / v_exp [n_pages, H, page], unit stride along the page.  Magnitudes beyond 1.875 * 2^15 (f16) or
+ * 1.875 * 2^127 (bf16), infinities among them, are stored as that; NaN stays NaN.
+ *
+ * vqa_paged_write: rows k, v [T,H,D] of the new tokens into their places (no two sequences of a call may write to the
+ *   same page).  strides[0..14] = k(t,h) v(t,h) k_pages(p,h,n) v_pages(p,h,n) k_exp(p,h) v_exp(p,h) table(s).
+ * vqa_paged_read: rows 0 .. n - 1 of every sequence as plain tensors k, v [S,H,n,D], zeros from kv_lens[s] on.
+ *   strides[0..16] = k_pages(p,h,n) v_pages(p,h,n) k_exp(p,h) v_exp(p,h) table(s) k(s,h,n) v(s,h,n).  S <= 65535.
+ * vqa_paged_attn: q [T,Hq,D] of the new tokens (Hq a multiple of Hkv; query head h reads key head h / (Hq / Hkv)) over
+ *   the cache, which already holds their keys: row t of sequence s, at position i, sees the keys j <= i with
+ *   i - j <= window (window < 0: no limit) when causal, else every key of its sequence.  One token per sequence is a
+ *   generation step, many are a chunk of a prompt, and one call takes both.  out [T,Hq,D], lse [T,Hq] contiguous
+ *   float, base 2, nullable; a row that sees no key gets 0 / -inf.  What hidden keys and values hold (infinities, NaN,
+ *   anything) never reaches a row.  max_q: the most new rows any sequence has, if the caller knows, else T; it only steers the
+ *   choice of kernels and the size of the workspace, results are right whatever it says.
+ *   strides[0..14] = q(t,h) k_pages(p,h,n) v_pages(p,h,n) k_exp(p,h) v_exp(p,h) table(s) out(t,h).
+ *   workspace: >= vqa_paged_attn_workspace_bytes(...) bytes, 256-byte aligned.
+ * D in {64, 128}.  Rows of every tensor 16-byte aligned.  The reference keeps dense caches only (ops/attn_rerope.py:19-113)
+ * and refuses a second chunk (ops/attn_vq.py:247); these entry points have no counterpart there.
+ * ------------------------------------------------------------------------------------------------------------------ */
+#define VQA_PAGED_WRITE_NUM_STRIDES 15
+#define VQA_PAGED_READ_NUM_STRIDES 17
+#define VQA_PAGED_ATTN_NUM_STRIDES 15
+
+int vqa_paged_write_bf16(const void* k, const void* v, void* k_pages, void* v_pages, uint8_t* k_exp, uint8_t* v_exp,
+                         const int32_t* block_table, const int32_t* cu_q, const int32_t* kv_lens, int T, int S, int H,
+                         int D, int page, int n_pages, int width, int e4m3, const int64_t* strides,
+                         vqa_stream_t stream);
+
+int vqa_paged_read_bf16(const void* k_pages, const void* v_pages, const uint8_t* k_exp, const uint8_t* v_exp,
+                        const int32_t* block_table, const int32_t* kv_lens, void* k, void* v, int S, int H, int n, int D,
+                        int page, int n_pages, int width, int e4m3, const int64_t* strides, vqa_stream_t stream);
+
+int vqa_paged_attn_bf16(const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_exp,
+                        const uint8_t* v_exp, const int32_t* block_table, const int32_t* cu_q, const int32_t* kv_lens,
+                        void* out, float* lse, void* workspace, size_t workspace_bytes, int T, int S, int Hq, int Hkv,
+                        int D, int page, int n_pages, int width, int e4m3, const int64_t* strides, int causal, int window,
+                        int max_q, float sm_scale, vqa_stream_t stream);
+
+int vqa_paged_write_f16(const void* k, const void* v, void* k_pages, void* v_pages, uint8_t* k_exp, uint8_t* v_exp,
+                         const int32_t* block_table, const int32_t* cu_q, const int32_t* kv_lens, int T, int S, int H,
+                         int D, int page, int n_pages, int width, int e4m3, const int64_t* strides,
+                         vqa_stream_t stream);
+
+int vqa_paged_read_f16(const void* k_pages, const void* v_pages, const uint8_t* k_exp, const uint8_t* v_exp,
+                        const int32_t* block_table, const int32_t* kv_lens, void* k, void* v, int S, int H, int n, int D,
+                        int page, int n_pages, int width, int e4m3, const int64_t* strides, vqa_stream_t stream);
+
+int vqa_paged_attn_f16(const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_exp,
+                        const uint8_t* v_exp, const int32_t* block_table, const int32_t* cu_q, const int32_t* kv_lens,
+                        void* out, float* lse, void* workspace, size_t workspace_bytes, int T, int S, int Hq, int Hkv,
+                        int D, int page, int n_pages, int width, int e4m3, const int64_t* strides, int causal, int window,
+                        int max_q, float sm_scale, vqa_stream_t stream);
+
+size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int max_q);
+
 #ifdef __cplusplus
 }
 #endif

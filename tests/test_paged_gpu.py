@@ -1,0 +1,414 @@
+"""Paged cache on the GPU against the 64-bit oracle: writing, reading back, and the attention of new tokens.
+
+Tolerances of the attention.  eps = half a step of the element type (bf16 2^-8, fp16 2^-11), u = 2^-24.  With A = sum of
+softmax * |v| and Z = the largest sum of |q_d k_d| * scale of a row:
+  * probabilities are rounded to the element type once: eps * A; the result is: eps * |out| <= eps * A;
+  * scores are fp32 sums of D exact products, in the order of the matrix pipe: (D + 2) * u * Z each, which moves a
+    weight by twice that (numerator and denominator), so 2 (D + 2) u Z * A; the long sums over N keys: 2 (N + 64) u * A, and exp2
+    itself a few u: 16 u * A;
+  * where the query is multiplied by the scale and rounded to the element type before the products (long chunks without
+    lse): another eps * Z on a score, 2 eps Z * A;
+  * fp16 has a smallest step of 2^-24: half of it per probability and result, N * 2^-25 * max|v| + 2^-25.
+The log-sum-exp is fp32 throughout: ((D + 2) Z + 2 (N + 64) + 16) * log2(e) * u, plus 2 u |lse|.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import paged as O
+from vqtree_amd.ops import paged_cache as P
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0**-24
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+class Cache:
+    """A random cache on the CPU (pools, exponents, table, lengths) and its copy on the GPU."""
+
+    def __init__(self, new, past, *, Hkv=2, G=1, D=128, page=16, dtype=torch.bfloat16, e4m3=False, seed=0, extra=0,
+                 spread=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.new, self.lens = list(new), [a + b for a, b in zip(new, past)]
+        self.Hkv, self.G, self.D, self.page, self.dtype, self.e4m3 = Hkv, G, D, page, dtype, e4m3
+        need = [-(-n // page) for n in self.lens]
+        n_pages = sum(need) + 2 + extra
+        width = max(need + [1]) + 1
+        order = torch.randperm(n_pages, generator=g).tolist()
+        self.table = torch.full((len(new), width), -1, dtype=torch.int32)
+        for s, n in enumerate(need):
+            for c in range(n):
+                self.table[s, c] = order.pop()
+        self.free = order
+        pools = []
+        for k in range(2):
+            x = torch.randn(n_pages, Hkv, page, D, generator=g) * (spread if k == 0 else 1.0)
+            if e4m3:
+                byte = torch.randint(118, 122, (n_pages, Hkv, page), generator=g, dtype=torch.int32)
+                pools += [(x * 32).to(torch.float8_e4m3fn), byte.to(torch.uint8)]  # values around 2^5 * 2^-7
+            else:
+                pools += [x.to(dtype), None]
+        self.k, self.k_exp, self.v, self.v_exp = pools
+        T = sum(new)
+        self.q = torch.randn(T, Hkv * G, D, generator=g).to(dtype)
+        self.cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32)
+        self.kv_lens = torch.tensor(self.lens, dtype=torch.int32)
+
+    def exps(self, dev=None):
+        if not self.e4m3:
+            return {}
+        return {"k_exp": self.k_exp.to(dev or "cpu"), "v_exp": self.v_exp.to(dev or "cpu")}
+
+    def attend(self, q=None, **kw):
+        q = self.q.to(DEV) if q is None else q
+        return P.attn_paged(q, self.k.to(DEV), self.v.to(DEV), self.table.to(DEV), self.cu.to(DEV), self.kv_lens.to(DEV),
+                            **self.exps(DEV), **kw)
+
+    def want(self, **kw):
+        return O.paged_attention(self.q, self.k, self.v, self.table, self.cu, self.kv_lens, **self.exps(), **kw)
+
+    def check(self, causal=True, window=None, lse=True, softmax_scale=None, max_q_len=None):
+        print("case", self.new, self.lens, self.Hkv, self.G, self.D, self.page, self.dtype, self.e4m3, causal, window, lse,
+              max_q_len, flush=True)
+        got = self.attend(causal=causal, window=window, return_lse=lse, softmax_scale=softmax_scale, max_q_len=max_q_len)
+        torch.cuda.synchronize()
+        compare(got if lse else (got, None), self.want(causal=causal, window=window, softmax_scale=softmax_scale), self,
+                prescaled=not lse)
+
+
+def compare(got, want, c, prescaled=False, rows=slice(None)):
+    out, lse = got
+    w_out, w_lse, A, Z = (x[rows] for x in want)
+    eps = torch.finfo(c.dtype).eps / 2
+    N, D = max(c.lens + [1]), c.D
+    Z = Z[..., None]
+    tol = (2 * eps + (2 * (D + 2) * Z + 2 * (N + 64) + 16) * U + (2 * eps * Z if prescaled else 0)) * A
+    if c.dtype == torch.float16:
+        tol = tol + N * 2.0**-25 * float(c.v.float().abs().nan_to_num(0, 0, 0).max()) + 2.0**-25
+    err = (out.double().cpu()[rows] - w_out).abs()
+    assert torch.isfinite(err).all(), "non-finite output"
+    assert (err <= tol).all(), f"out: {float((err / tol.clamp(min=1e-30)).max()):.3g} of the tolerance, max err {float(err.max()):.3g}"
+    if lse is not None:
+        lse = lse.double().cpu()[rows]
+        same = lse == w_lse  # both -inf
+        tol = ((D + 2) * Z[..., 0] + 2 * (N + 64) + 16) * 1.4427 * U + 2 * U * w_lse.abs()
+        bad = ~(same | ((lse - w_lse).abs() <= tol))
+        assert not bad.any(), f"lse: {int(bad.sum())} off, {float((lse - w_lse).abs().nan_to_num(0).max()):.3g}"
+
+
+FORMS = [("bf16", False, 128, 1, 16), ("bf16", True, 128, 4, 64), ("f16", False, 64, 4, 32), ("f16", True, 64, 1, 16),
+         ("bf16", False, 128, 8, 64), ("bf16", True, 64, 7, 128), ("f16", True, 128, 2, 256)]
+LENGTHS = {
+    "single": ([1, 1, 1], [0, 15, 300]),
+    "long_single": ([1], [5000]),
+    "few": ([5, 3, 1, 8], [60, 0, 64, 1000]),
+    "chunk": ([150], [333]),
+    "first_chunk": ([257], [0]),
+    "mixed": ([70, 1, 0, 33, 1], [130, 640, 12, 0, 63]),
+    "nothing": ([0, 0], [0, 77]),
+}
+
+
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: f"{f[0]}-{'e4m3' if f[1] else '16'}-d{f[2]}-g{f[3]}-p{f[4]}")
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+def test_attention(lengths, form):
+    new, past = LENGTHS[lengths]
+    dtype, e4m3, D, G, page = form
+    c = Cache(new, past, Hkv=3 if G < 4 else 2, G=G, D=D, page=page, dtype=DTYPES[dtype], e4m3=e4m3, seed=len(lengths))
+    if c.q.shape[0] == 0:
+        out, lse = c.attend(return_lse=True)
+        assert out.shape == c.q.shape and lse.shape == c.q.shape[:2]
+        return
+    c.check()
+    c.check(lse=False, max_q_len=max(new))
+    c.check(window=40)
+    c.check(causal=False)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# writing and reading
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("D,page,H", [(128, 16, 3), (64, 64, 1)])
+def test_write_then_read(dtype, e4m3, D, page, H):
+    dt = DTYPES[dtype]
+    new, past = [3, 0, 65, 1, 40], [14, 5, 0, 200, 63]
+    c = Cache(new, past, Hkv=H, D=D, page=page, dtype=dt, e4m3=e4m3, seed=3)
+    g = torch.Generator().manual_seed(4)
+    T = sum(new)
+    buf = torch.randn(T + 9, 3 * H * D, generator=g)  # columns of a projection; 9 rows behind the last sequence
+    buf[:T] *= torch.logspace(-6, 3, T)[:, None]
+    buf[2], buf[7, :D] = 0, 0
+    buf[5, H * D + 3], buf[6, H * D + 5], buf[8, 2 * H * D + 1] = math.inf, -math.inf, math.nan
+    buf[9, H * D] = 65504.0
+    buf[10, :] *= 1e-6
+    buf = buf.to(dt)
+    k, v = buf[:, H * D:2 * H * D].view(-1, H, D), buf[:, 2 * H * D:].view(-1, H, D)
+    gpu = [x.to(DEV) if x is not None else None for x in (c.k, c.v, c.k_exp, c.v_exp)]
+    kg, vg = (x.view(-1, H, D) for x in buf.to(DEV)[:, H * D:].split(H * D, 1))
+    assert not kg.is_contiguous()
+    exps = dict(k_exp=gpu[2], v_exp=gpu[3]) if e4m3 else {}
+    P.paged_write(kg, vg, gpu[0], gpu[1], c.table.to(DEV), c.cu.to(DEV), c.kv_lens.to(DEV), **exps)
+    torch.cuda.synchronize()
+    want = [c.k.clone(), c.v.clone(), None if c.k_exp is None else c.k_exp.clone(), None if c.v_exp is None else c.v_exp.clone()]
+    for s, n in enumerate(new):
+        for t in range(n):
+            j = c.lens[s] - n + t
+            p, o, row = int(c.table[s, j // page]), j % page, int(c.cu[s]) + t
+            for pages, exp, x in ((want[0], want[2], k), (want[1], want[3], v)):
+                if exp is None:
+                    pages[p, :, o] = x[row]
+                else:
+                    values, byte = O.quantise_rows(x[row])
+                    scaled = torch.ldexp(values, 127 - byte.int().unsqueeze(-1))
+                    pages.view(torch.uint8)[p, :, o] = scaled.float().to(torch.float8_e4m3fn).view(torch.uint8)
+                    exp[p, :, o] = byte
+    bits = torch.uint8 if e4m3 else torch.int16
+    for a, b in zip(gpu[:2], want[:2]):
+        a, b = a.cpu().view(bits), b.view(bits)
+        same = a == b
+        if e4m3:  # a NaN keeps no sign
+            same |= ((a & 0x7F) == 0x7F) & ((b & 0x7F) == 0x7F)
+        assert same.all(), f"{int((~same).sum())} elements differ"
+    if e4m3:
+        assert torch.equal(gpu[2].cpu(), want[2]) and torch.equal(gpu[3].cpu(), want[3])
+    # and back
+    n = max(c.lens) + 3
+    rk, rv = P.paged_read(gpu[0], gpu[1], c.table.to(DEV), c.kv_lens.to(DEV), n, dtype=dt, **exps)
+    for got, pages, exp in ((rk, want[0], want[2]), (rv, want[1], want[3])):
+        for s in range(len(new)):
+            x, _ = O.rows_of(pages, exp, c.table[s], c.lens[s])
+            full = torch.zeros(H, n, D, dtype=torch.float64)
+            full[:, :c.lens[s]] = x
+            assert torch.equal(got[s].cpu().nan_to_num(7.0), full.to(dt).nan_to_num(7.0))
+            assert torch.isfinite(full).sum() == torch.isfinite(got[s]).sum().cpu()
+
+
+def test_every_e4m3_number_reads_back_exactly():
+    """256 bit patterns under exponents 2^-126 .. 2^120, against the exact product rounded once."""
+    page, D = 256, 64
+    pages = torch.arange(256, dtype=torch.uint8).repeat(page * D // 256).view(1, 1, page, D)
+    byte = torch.arange(256, dtype=torch.int32).clamp(1, 247).to(torch.uint8).view(1, 1, page)
+    pages8 = pages.view(torch.float8_e4m3fn)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32), torch.tensor([page], dtype=torch.int32)
+    exact = torch.ldexp(pages8.float().double(), byte.int().unsqueeze(-1) - 127)
+    for dt in (torch.bfloat16, torch.float16):
+        k, v = P.paged_read(pages8.to(DEV), pages8.to(DEV), table.to(DEV), lens.to(DEV), page, k_exp=byte.to(DEV),
+                            v_exp=byte.to(DEV), dtype=dt)
+        want = exact.to(dt)  # (torch rounds a double to 16 bits once)
+        ok = exact.abs() <= torch.finfo(dt).max
+        normal = ok & ((exact == 0) | (exact.abs() >= torch.finfo(dt).tiny))
+        for got in (k.cpu(), v.cpu()):
+            assert torch.equal(got[normal], want[normal])
+            tiny = ok & ~normal  # results below the normal numbers: within a step of the smallest number, or flushed to it
+            step = torch.finfo(dt).tiny * torch.finfo(dt).eps
+            bound = torch.finfo(dt).tiny if dt == torch.bfloat16 else step
+            assert ((got[tiny].double() - exact[tiny]).abs() <= bound).all()
+            nan = torch.isnan(exact)
+            assert torch.isnan(got[nan]).all()
+
+
+def test_rows_that_have_no_place_are_skipped():
+    """Behind the last sequence, before position 0, behind the table, on pages that are not there: nothing is written."""
+    H, D, page = 2, 64, 16
+    k = torch.randn(40, H, D, device=DEV).to(torch.bfloat16)
+    pool = torch.zeros(4, H, page, D, dtype=torch.bfloat16, device=DEV)
+    k_pages, v_pages = pool.clone(), pool.clone()
+    table = torch.tensor([[1, 99], [-5, 2], [3, 3]], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 20, 30, 33], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([20, 26, 34], dtype=torch.int32, device=DEV)  # the third has places 31, 32, 33: two behind the table
+    P.paged_write(k, k, k_pages, v_pages, table, cu, lens)
+    want = pool.clone()
+    want[1] = k[:16].transpose(0, 1)       # sequence 0: positions 0 .. 15 on page 1, 16 .. 19 on no page
+    want[2, :, :10] = k[20:30].transpose(0, 1)  # sequence 1: positions 16 .. 25
+    want[3, :, 15] = k[30]
+    assert torch.equal(k_pages, want) and torch.equal(v_pages, want)
+    P.paged_write(k, k, k_pages, v_pages, table, cu, torch.tensor([-3, 4, 2], dtype=torch.int32, device=DEV))
+    want[3, :, 0], want[3, :, 1] = k[31], k[32]  # sequence 1: no page; sequence 2: row 30 would be at position -1
+    assert torch.equal(k_pages, want)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# hidden places, missing pages, odd metadata
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new,past", [([1, 1], [20, 333]), ([130], [70]), ([300, 5], [0, 900])])
+def test_hidden_places_may_hold_anything(e4m3, new, past):
+    """NaN and infinities in unused places of the last page, in keys above the causal limit and below the window, and on
+    pages nobody reads."""
+    c = Cache(new, past, D=128, page=64, e4m3=e4m3, seed=9)
+    clean = c.want(window=50)
+    bad = 0x7F if e4m3 else None
+    for s, n in enumerate(c.lens):
+        for j in range(0, (c.table.shape[1] - 1) * 64):
+            p = int(c.table[s, j // 64])
+            first = c.lens[s] - new[s] - 50  # the first row's window starts here
+            if p >= 0 and (j >= n or j < first):
+                for pool in (c.k, c.v):
+                    if bad is None:
+                        pool[p, :, j % 64] = math.nan if j % 2 else math.inf
+                    else:
+                        pool.view(torch.uint8)[p, :, j % 64] = bad
+    for p in c.free:
+        for pool in (c.k, c.v):
+            pool.view(torch.uint8)[p] = 0x7F
+    compare(c.attend(window=50, return_lse=True), clean, c)
+
+
+@pytest.mark.parametrize("new", [7, 200])
+def test_a_later_tokens_nan_does_not_reach_earlier_rows(new):
+    c = Cache([new], [90], D=64, page=16, G=2, seed=2)
+    clean = c.want()
+    first = c.lens[0] - 3  # the last three tokens' values are poison
+    for j in range(first, c.lens[0]):
+        c.v[int(c.table[0, j // 16]), :, j % 16] = math.inf if j == first else math.nan
+    out, lse = c.attend(return_lse=True)
+    compare((out, lse), clean, c, rows=slice(0, new - 3))
+    assert torch.isinf(out[new - 3]).all() and torch.isnan(out[new - 2:]).all()
+
+
+def test_missing_pages_and_odd_lengths():
+    c = Cache([1, 40, 3, 2], [300, 100, 0, 700], D=128, page=16, G=2, seed=5)
+    c.table[0, 3], c.table[0, 18], c.table[1, 0], c.table[3, 1] = -1, c.k.shape[0], 2**31 - 1, -(2**31)
+    c.table[2, :] = -1           # nothing there at all
+    c.kv_lens[3] = 10_000        # more keys than the table has room for: the rows stand behind them all
+    c.lens[3] = 10_000
+    got = c.attend(return_lse=True)
+    want = c.want()
+    compare(got, want, c)
+    assert (got[0][41:44] == 0).all() and torch.isinf(got[1][41:44]).all()
+    got = c.attend(return_lse=True, window=20)
+    compare(got, c.want(window=20), c)
+    c.kv_lens[1], c.lens[1] = 25, 25  # fewer keys than new rows: the first 15 see nothing
+    got = c.attend(return_lse=True)
+    compare(got, c.want(), c)
+    assert (got[0][1:16] == 0).all() and torch.isinf(got[1][1:16]).all()
+    c.kv_lens[1], c.lens[1] = -7, 0
+    compare(c.attend(return_lse=True), c.want(), c)
+
+
+@pytest.mark.parametrize("new", [[1, 2], [90, 40]])
+def test_rows_behind_the_last_sequence_are_left_alone(new):
+    c = Cache(new, [100, 30], D=64, G=4, seed=6)
+    T = sum(new)
+    q = torch.cat([c.q, torch.full((37, 8, 64), math.nan, dtype=c.dtype)]).to(DEV)
+    out = torch.full((T + 37, 8, 64), 5.0, dtype=c.dtype, device=DEV)
+    got, lse = c.attend(q, out=out, return_lse=True)
+    assert got is out and (out[T:] == 5).all()
+    compare((out[:T], lse[:T]), c.want(), c)
+
+
+def test_numbers_out_of_range_do_no_harm():
+    """cu_q that decreases or runs past the rows: memory stays in bounds; rows of well-formed sequences come out right."""
+    c = Cache([4, 40, 4], [50, 20, 30], D=64, seed=7)
+    c.cu = torch.tensor([0, 4, 44, 2**31 - 1], dtype=torch.int32)
+    out = c.attend()
+    assert out.shape == c.q.shape and torch.isfinite(out.float()).all()
+    c.cu = torch.tensor([0, -5, 2**31 - 1, -(2**31)], dtype=torch.int32)
+    c.attend()
+    torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# layouts, streams, graphs, a whole run
+@pytest.mark.parametrize("new", [[1, 1], [100, 3]])
+def test_strided_tensors(new):
+    """q as columns of a projection, out as rows of a wider buffer, key and value pages interleaved in one pool."""
+    c = Cache(new, [200, 31], D=128, G=4, Hkv=2, page=32, seed=8)
+    T = sum(new)
+    kv = torch.stack([c.k, c.v], 1).to(DEV)  # [pages, 2, H, page, D]
+    buf = torch.randn(T, 12, 128, device=DEV).to(c.dtype)
+    buf[:, :8] = c.q.to(DEV)
+    wide = torch.zeros(T, 16, 128, dtype=c.dtype, device=DEV)
+    out, lse = P.attn_paged(buf[:, :8], kv[:, 0], kv[:, 1], c.table.to(DEV)[:, :-1], c.cu.to(DEV), c.kv_lens.to(DEV),
+                            out=wide[:, 4:12], return_lse=True)
+    compare((out, lse), c.want(), c)
+    assert (wide[:, :4] == 0).all() and (wide[:, 12:] == 0).all()
+    # a transposed query (last dimension not contiguous) is copied
+    qt = c.q.to(DEV).transpose(1, 2).contiguous().transpose(1, 2)
+    compare(P.attn_paged(qt, kv[:, 0], kv[:, 1], c.table.to(DEV), c.cu.to(DEV), c.kv_lens.to(DEV), return_lse=True), c.want(), c)
+
+
+def test_another_stream_and_two_calls_at_once():
+    a, b = Cache([1, 1], [3000, 700], seed=10, G=2), Cache([80], [900], seed=11, G=2, e4m3=True)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    gots = []
+    args = [(c.q.to(DEV), c.k.to(DEV), c.v.to(DEV), c.table.to(DEV), c.cu.to(DEV), c.kv_lens.to(DEV), c.exps(DEV)) for c in (a, b)]
+    torch.cuda.synchronize()
+    for stream, (*x, e) in zip((sa, sb), args):
+        with torch.cuda.stream(stream):
+            gots.append(P.attn_paged(*x, **e, return_lse=True))
+    torch.cuda.synchronize()
+    compare(gots[0], a.want(), a)
+    compare(gots[1], b.want(), b)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [130, 1, 20]])
+def test_recorded_step_replays_on_new_lengths(new):
+    """A whole step -- write, then attend -- recorded once: lengths, tables and rows change between the replays."""
+    H, G, D, page, S, width = 2, 2, 128, 16, 3, 64
+    T = sum(new)
+    g = torch.Generator().manual_seed(12)
+    pools = [torch.zeros(S * width, H, page, D, dtype=torch.float8_e4m3fn, device=DEV) for _ in range(2)]
+    exps = [torch.ones(S * width, H, page, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    table = torch.randperm(S * width, generator=g).view(S, width).to(torch.int32).to(DEV)
+    cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+    lens = torch.tensor(new, dtype=torch.int32, device=DEV)
+    q, k, v = (torch.zeros(T, h, D, dtype=torch.bfloat16, device=DEV) for h in (H * G, H, H))
+    e = dict(k_exp=exps[0], v_exp=exps[1])
+
+    def step():
+        P.paged_write(k, v, *pools, table, cu, lens, **e)
+        return P.attn_paged(q, *pools, table, cu, lens, **e, return_lse=True)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = step()
+    for i in range(4):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g))
+        lens.copy_(torch.tensor([n * (i + 1) + 100 * s * (i % 2) for s, n in enumerate(new)], dtype=torch.int32))
+        graph.replay()
+        got = out.clone(), lse.clone()
+        again = step()  # (writes the same rows to the same places)
+        assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+        c = Cache([1], [1])
+        c.lens, c.D, c.dtype = lens.tolist(), D, torch.bfloat16
+        want = O.paged_attention(q.cpu(), pools[0].cpu(), pools[1].cpu(), table.cpu(), cu.cpu(), lens.cpu(),
+                                 k_exp=exps[0].cpu(), v_exp=exps[1].cpu())
+        compare(got, want, c)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_a_run_of_steps(e4m3):
+    """A prompt in three chunks, then single tokens, two sequences joining on the way: after every step the attention equals
+    that over everything written so far, and the cache reads back as the tensors a dense operator takes."""
+    from vqtree_amd.ops.attn_vq import attn_exact_decode
+
+    H, G, D, page, width = 2, 2, 64, 16, 24
+    g = torch.Generator().manual_seed(13)
+    dt = torch.bfloat16
+    pools = [torch.zeros(3 * width, H, page, D, dtype=torch.float8_e4m3fn if e4m3 else dt, device=DEV) for _ in range(2)]
+    e = dict(zip(("k_exp", "v_exp"), (torch.ones(3 * width, H, page, dtype=torch.uint8, device=DEV) for _ in range(2)))) if e4m3 else {}
+    table = torch.randperm(3 * width, generator=g).view(3, width).to(torch.int32).to(DEV)
+    have = [0, 0, 0]
+    for new in ([100, 0, 0], [61, 33, 0], [17, 1, 9], [1, 1, 1], [1, 1, 1], [4, 0, 2]):
+        T = sum(new)
+        q, k, v = (torch.randn(T, h, D, generator=g).to(dt).to(DEV) for h in (H * G, H, H))
+        have = [a + b for a, b in zip(have, new)]
+        cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+        lens = torch.tensor(have, dtype=torch.int32, device=DEV)
+        P.paged_write(k, v, *pools, table, cu, lens, **e)
+        got = P.attn_paged(q, *pools, table, cu, lens, **e, return_lse=True)
+        c = Cache([1], [1], dtype=dt, D=D)
+        c.lens = have
+        cpu = {n: x.cpu() for n, x in e.items()}
+        compare(got, O.paged_attention(q.cpu(), pools[0].cpu(), pools[1].cpu(), table.cpu(), cu.cpu(), lens.cpu(), **cpu), c)
+    # the last token of sequence 0, by the dense operator on the cache read back
+    k, v = P.paged_read(*pools, table, lens, have[0], dtype=dt, **e)
+    last = q[new[0] - 1].view(1, H * G, 1, D)
+    dense = attn_exact_decode(last, k[:1].repeat_interleave(G, 1), v[:1].repeat_interleave(G, 1))
+    assert (dense[0, :, 0].float() - got[0][new[0] - 1].float()).abs().max() <= 2.0**-6

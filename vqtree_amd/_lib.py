@@ -68,6 +68,13 @@ SIGNATURES = {
     "vqa_preprocess_f16": (c_int, [_P] * 7 + [c_size_t] + [c_int] * 5 + [_STRIDES, _P]),
     "vqa_preprocess_state_bf16": (c_int, [_P] * 9 + [c_size_t] + [c_int] * 5 + [_STRIDES, _P]),
     "vqa_preprocess_state_f16": (c_int, [_P] * 9 + [c_size_t] + [c_int] * 5 + [_STRIDES, _P]),
+    "vqa_paged_write_bf16": (c_int, [_P] * 9 + [c_int] * 8 + [_STRIDES, _P]),
+    "vqa_paged_write_f16": (c_int, [_P] * 9 + [c_int] * 8 + [_STRIDES, _P]),
+    "vqa_paged_read_bf16": (c_int, [_P] * 8 + [c_int] * 8 + [_STRIDES, _P]),
+    "vqa_paged_read_f16": (c_int, [_P] * 8 + [c_int] * 8 + [_STRIDES, _P]),
+    "vqa_paged_attn_bf16": (c_int, [_P] * 11 + [c_size_t] + [c_int] * 9 + [_STRIDES, c_int, c_int, c_int, c_float, _P]),
+    "vqa_paged_attn_f16": (c_int, [_P] * 11 + [c_size_t] + [c_int] * 9 + [_STRIDES, c_int, c_int, c_int, c_float, _P]),
+    "vqa_paged_attn_workspace_bytes": (c_size_t, [c_int] * 6),
 }
 
 
