@@ -3,7 +3,7 @@
 
 extern "C" {
 
-int vqa_version(void) { return 110; /* 0.1.1: vqa_decode_roped_*, window kinds of the pipelined core */ }
+int vqa_version(void) { return 120; /* 0.1.2: vqa_paged_* */ }
 
 const char* vqa_strerror(int status) {
     switch (status) {

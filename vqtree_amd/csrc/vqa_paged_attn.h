@@ -6,6 +6,8 @@
 // lse = -inf.
 #pragma once
 
+#include <mutex>
+
 #include "vqa_paged.h"
 
 namespace vqa {
@@ -44,7 +46,7 @@ struct RowState {
 };
 
 template <typename Tag, int D, bool kE4m3>
-__device__ __noinline__ void row_by_lanes(const AttnArgs& a, int s, int h, const uint16_t* q, int lo, int hi,
+__device__ __forceinline__ void row_by_lanes(const AttnArgs& a, int s, int h, const uint16_t* q, int lo, int hi,
                                           RowState<D>& st, int lane) {
     constexpr int E = D / 64;
     st.m = -INFINITY;
@@ -140,6 +142,138 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& 
     if (a.lse != nullptr && lane == 0)
         a.lse[(int64_t)row * a.Hq + hq] = st.l == 0.f ? -INFINITY : st.m + fast_log2(st.l);
 }
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Work units.  The new rows of a sequence and the G query heads of a key head are one list of n * G rows (row r: new token
+// r / G, head r % G of the group), cut into tiles; the keys a sequence's rows see are cut into splits.  A unit is one tile
+// and one split of one sequence.  How long a split is follows from the lengths found on the device: the work of the call
+// over the number of workgroups that fill the chip, so a batch of unequal lengths is spread evenly and a recorded call
+// adapts to new ones.  Every kernel of a call computes the same plan from the same numbers.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int kKeyStep = 64;  // splits begin and end at multiples of this many keys
+
+struct Plan {
+    int rows;       // rows of a tile
+    int lo, hi;     // sequences with lo <= n * G <= hi belong to this kernel
+    int max_tiles;  // the grid and the workspace are made for this many tiles (of one key head) ...
+    int units;      // ... and units; more of either (a wrong hint): no splits
+    int per_head;   // workgroups worth having per key head
+    int min_steps;  // shortest split, in key steps
+    float* o;       // partial results [unit * Hkv + head][rows][D], unnormalised
+    float* ml;      // [..][rows][2]: maximum (base 2, scaled) and sum
+};
+
+struct Share {  // what one sequence brings
+    int tiles, first, steps;  // row tiles; first key step its rows see; number of key steps
+};
+__device__ __forceinline__ Share share_of(const AttnArgs& a, const Plan& p, int s) {
+    if (s >= a.g.S) return {0, 0, 0};
+    const Seq q = seq_of(a.g, s);
+    const int64_t rows = (int64_t)q.n * a.G;
+    if (rows < 1 || rows < p.lo || rows > p.hi) return {0, 0, 0};
+    const Range r0 = visible(a, q, 0);
+    const int hi = visible(a, q, q.n - 1).hi;
+    Share x;
+    x.tiles = (int)((rows + p.rows - 1) / p.rows);
+    x.first = r0.lo / kKeyStep;
+    x.steps = max(0, (hi + kKeyStep - 1) / kKeyStep - x.first);
+    return x;
+}
+
+__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t lo = __shfl_xor((uint32_t)x, o, 64), hi = __shfl_xor((uint32_t)(x >> 32), o, 64);
+        x += (int64_t)(((uint64_t)hi << 32) | lo);
+    }
+    return x;
+}
+
+// Key steps per split of this call (0x7fffffff: no splits), the same in every wave.
+__device__ __forceinline__ int split_steps(const AttnArgs& a, const Plan& p, int lane) {
+    int64_t work = 0, tiles = 0;
+    for (int base = 0; base < a.g.S; base += kWave) {
+        const Share x = share_of(a, p, base + lane);
+        work += (int64_t)x.tiles * x.steps;
+        tiles += x.tiles;
+    }
+    work = wave_sum64(work);
+    tiles = wave_sum64(tiles);
+    if (tiles > p.max_tiles || p.per_head < 1) return 0x7fffffff;
+    const int64_t per = (work + p.per_head - 1) / p.per_head;
+    // sum over tiles of ceil(steps / per) <= work / per + tiles <= per_head + max_tiles = units
+    return (int)max((int64_t)p.min_steps, per < 0x7fffffff ? per : 0x7fffffff);
+}
+__device__ __forceinline__ int splits_of(const Share& x, int per) {
+    return x.steps <= per ? 1 : (x.steps + per - 1) / per;
+}
+
+struct Unit {
+    int s, tile, split, n_splits, slot;  // slot: number of the unit (its place in the workspace)
+    int first, steps;                    // the sequence's key steps
+};
+// unit x of the call, s = -1 if there is none
+__device__ __forceinline__ Unit find_unit(const AttnArgs& a, const Plan& p, int per, int64_t x, int lane) {
+    Unit u;
+    u.s = -1;
+    int64_t before = 0;
+    for (int base = 0; base < a.g.S; base += kWave) {
+        const Share h = share_of(a, p, base + lane);
+        const int n_splits = splits_of(h, per);
+        // (tiles * splits of one sequence fits 32 bits: with splits there are at most `units` of them, without it is the
+        // number of tiles)
+        const int mine = h.tiles * n_splits;
+        int64_t sum = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t lo = __shfl_up((uint32_t)sum, o, 64), hi = __shfl_up((uint32_t)(sum >> 32), o, 64);
+            if (lane >= o) sum += (int64_t)(((uint64_t)hi << 32) | lo);
+        }
+        const bool here = x < before + sum;
+        const uint64_t vote = __builtin_amdgcn_ballot_w64(here);
+        if (vote) {
+            const int at = __builtin_ctzll(vote);
+            const int64_t start = before + sum - mine;
+            const int64_t rest = x - start;
+            u.s = base + at;
+            const int local = __shfl((int)rest, at, 64);
+            u.n_splits = __shfl(n_splits, at, 64);
+            u.first = __shfl(h.first, at, 64);
+            u.steps = __shfl(h.steps, at, 64);
+            u.tile = local / u.n_splits;
+            u.split = local % u.n_splits;
+            u.slot = (int)x;
+            return u;
+        }
+        before += wave_sum64(mine);
+    }
+    return u;
+}
+// keys [first, last) of a split: the steps are dealt out evenly
+__device__ __forceinline__ Range split_keys(const Unit& u) {
+    const int a = (int)((int64_t)u.steps * u.split / u.n_splits), b = (int)((int64_t)u.steps * (u.split + 1) / u.n_splits);
+    return {(u.first + a) * kKeyStep, (u.first + b) * kKeyStep};
+}
+
+// Kernels that use more than 64 KB of LDS need the limit raised once per device: the one that owns the operands.
+template <auto kKernel>
+int raise_lds(const void* operand, int bytes) {
+    static std::mutex mutex;
+    static bool raised[kMaxDevices] = {};
+    int dev = 0;
+    if (int rc = device_of_pointer(operand, &dev)) return rc;
+    std::lock_guard<std::mutex> lock(mutex);
+    if (!raised[dev]) {
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+            hipSuccess)
+            return VQA_ERR_LAUNCH_FAILED;
+        raised[dev] = true;
+    }
+    return VQA_OK;
+}
+
+template <typename Tag>
+int launch_few(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream);
 
 }  // namespace paged
 }  // namespace vqa

@@ -6,28 +6,113 @@
 namespace vqa {
 namespace paged {
 
-// One wave per row and query head.
-template <typename Tag, int D, bool kE4m3>
-__global__ __launch_bounds__(256) void rows_kernel(AttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = (int)(id / a.Hq), hq = (int)(id % a.Hq);
-    if (row >= a.g.T) return;
+// Joins the splits of a row: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.  One workgroup per row and query head,
+// its waves share the splits (their partial rows are 512 bytes each, so what counts is how many are in flight).
+constexpr int kJoinWaves = 4;
+
+template <typename Tag, int D>
+__global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan p) {
+    constexpr int E = D / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = (int)(blockIdx.x / (unsigned)a.Hq), hq = (int)(blockIdx.x % (unsigned)a.Hq);
     const int s = find_seq(a.g, row, lane);
     if (s >= a.g.S) return;
     const Seq q = seq_of(a.g, s);
     if (row < q.q0 || row >= q.q0 + q.n) return;
-    const Range r = visible(a, q, row - q.q0);
+    const int per = split_steps(a, p, lane);
+    const Share mine = share_of(a, p, s);
+    const int n_splits = splits_of(mine, per);
+    if (mine.tiles == 0 || n_splits == 1) return;  // (one split: the unit has stored the result itself)
+    int64_t slot = 0;
+    for (int base = 0; base < s; base += kWave) {
+        const Share x = share_of(a, p, min(base + lane, s));
+        slot += wave_sum64(base + lane < s ? (int64_t)x.tiles * splits_of(x, per) : 0);
+    }
+    const int h = hq / a.G, r = (row - q.q0) * a.G + hq % a.G;
+    slot += (int64_t)(r / p.rows) * n_splits;
+    const int64_t first = (slot * a.Hkv + h) * p.rows + r % p.rows, step = (int64_t)a.Hkv * p.rows;
+    float top = -INFINITY;
+    for (int i = lane; i < n_splits; i += 64) top = fmaxf(top, p.ml[(first + i * step) * 2]);
+    top = wave_max(top);
+    float o[E], l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int i = wave; i < n_splits; i += kJoinWaves) {
+        const int64_t at = first + i * step;
+        const float m = p.ml[at * 2];
+        const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
+        l += f * p.ml[at * 2 + 1];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += f * p.o[at * D + lane * E + e];
+    }
+    __shared__ float part[kJoinWaves][64][E + 1];
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[wave][lane][e] = o[e];
+    part[wave][lane][E] = l;
+    __syncthreads();
+    if (wave != 0) return;
     RowState<D> st;
-    row_by_lanes<Tag, D, kE4m3>(a, s, hq / a.G, a.q + (int64_t)row * a.q_st + (int64_t)hq * a.q_sh, r.lo, r.hi, st, lane);
+    st.m = top, st.l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) st.o[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) {
+        st.l += part[w][lane][E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) st.o[e] += part[w][lane][e];
+    }
     store_row<Tag, D>(a, st, row, hq, lane);
 }
 
-template <typename Tag, int D, bool kE4m3>
-int launch(const AttnArgs& a, hipStream_t stream) {
-    const int64_t blocks = ((int64_t)a.g.T * a.Hq + 3) / 4;
-    rows_kernel<Tag, D, kE4m3><<<dim3((unsigned)blocks), 256, 0, stream>>>(a);
-    return launch_status();
+// How a call is cut up (host side; the numbers of rows and keys themselves are known on the device only).
+struct Cut {
+    Plan few;
+    int64_t few_grid;
+    size_t bytes;  // workspace
+};
+
+constexpr int kFewUnits = 512;  // workgroups that fill the chip: two per compute unit
+
+inline size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
+
+inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q) {
+    const int G = Hq / Hkv;
+    Cut c{};
+    const int64_t most = (int64_t)std::max(1, std::min(max_q, T)) * G;  // rows of a sequence
+    Plan& p = c.few;
+    p.rows = most <= 16 ? 16 : 32;
+    p.lo = 1, p.hi = 0x7fffffff;
+    const int64_t seqs = std::min(S, T);
+    const int64_t tiles = std::min((int64_t)T * G / p.rows + seqs, seqs * ((most + p.rows - 1) / p.rows));
+    p.max_tiles = (int)std::min<int64_t>(tiles, 0x3fffffff);
+    p.per_head = tiles * Hkv >= kFewUnits ? 0 : (kFewUnits + Hkv - 1) / Hkv;
+    p.units = p.max_tiles + p.per_head;
+    p.min_steps = 4;
+    c.few_grid = (int64_t)p.units * Hkv;
+    if (p.per_head) {
+        const size_t rows = (size_t)p.units * Hkv * p.rows;
+        c.bytes = round256(rows * D * 4) + round256(rows * 8);
+    }
+    return c;
+}
+
+template <typename Tag>
+int run(AttnArgs& a, Cut& c, void* ws, int D, bool e4m3, hipStream_t stream) {
+    Plan& p = c.few;
+    const size_t rows = (size_t)p.units * a.Hkv * p.rows;
+    p.o = (float*)ws;
+    p.ml = (float*)((char*)ws + round256(rows * D * 4));
+    if (int rc = launch_few<Tag>(a, p, D, e4m3, c.few_grid, stream)) return rc;
+    if (p.per_head) {
+        const dim3 grid((unsigned)((int64_t)a.g.T * a.Hq));
+        if (D == 128)
+            join_kernel<Tag, 128><<<grid, kJoinWaves * 64, 0, stream>>>(a, p);
+        else
+            join_kernel<Tag, 64><<<grid, kJoinWaves * 64, 0, stream>>>(a, p);
+        return launch_status();
+    }
+    return VQA_OK;
 }
 
 template <typename Tag>
@@ -53,8 +138,12 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
     a.window = window < 0 ? 1 << 30 : std::min(window, 1 << 30);
     a.scale_log2e = scale * kLog2e;
     if (S == 0 || T == 0) return VQA_OK;
-    if (D == 128) return e4m3 ? launch<Tag, 128, true>(a, stream) : launch<Tag, 128, false>(a, stream);
-    return e4m3 ? launch<Tag, 64, true>(a, stream) : launch<Tag, 64, false>(a, stream);
+    Cut c = cut_call(T, S, Hq, Hkv, D, max_q);
+    if (c.few_grid > 0x7fffffff) return VQA_ERR_BAD_SHAPE;
+    if (c.bytes && ws == nullptr) return VQA_ERR_NULL_POINTER;
+    if (reinterpret_cast<uintptr_t>(ws) % 256) return VQA_ERR_MISALIGNED;
+    if (ws_bytes < c.bytes) return VQA_ERR_WORKSPACE_TOO_SMALL;
+    return run<Tag>(a, c, ws, D, e4m3 != 0, stream);
 }
 
 }  // namespace paged
@@ -62,7 +151,10 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
 
 extern "C" {
 
-size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int max_q) { return 0; }
+size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int max_q) {
+    if (T < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || (D != 64 && D != 128)) return 0;
+    return vqa::paged::cut_call(T, S, Hq, Hkv, D, max_q).bytes;
+}
 
 #define VQA_PAGED_ATTN(sfx, tag)                                                                                          \
     int vqa_paged_attn_##sfx(const void* q, const void* k_pages, const void* v_pages, const uint8_t* k_exp,              \
