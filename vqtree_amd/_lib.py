@@ -74,7 +74,7 @@ SIGNATURES = {
     "vqa_paged_read_f16": (c_int, [_P] * 8 + [c_int] * 8 + [_STRIDES, _P]),
     "vqa_paged_attn_bf16": (c_int, [_P] * 11 + [c_size_t] + [c_int] * 9 + [_STRIDES, c_int, c_int, c_int, c_float, _P]),
     "vqa_paged_attn_f16": (c_int, [_P] * 11 + [c_size_t] + [c_int] * 9 + [_STRIDES, c_int, c_int, c_int, c_float, _P]),
-    "vqa_paged_attn_workspace_bytes": (c_size_t, [c_int] * 6),
+    "vqa_paged_attn_workspace_bytes": (c_size_t, [c_int] * 10),
 }
 
 
@@ -113,6 +113,13 @@ def current_stream(device):
     import torch
 
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def raw_stream(device_index):
+    """The current stream of a device as the integer handle the entry points take (no stream object is made)."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def require_gpu(*tensors):

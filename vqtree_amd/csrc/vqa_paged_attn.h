@@ -144,116 +144,119 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Work units.  The new rows of a sequence and the G query heads of a key head are one list of n * G rows (row r: new token
-// r / G, head r % G of the group), cut into tiles; the keys a sequence's rows see are cut into splits.  A unit is one tile
-// and one split of one sequence.  How long a split is follows from the lengths found on the device: the work of the call
-// over the number of workgroups that fill the chip, so a batch of unequal lengths is spread evenly and a recorded call
-// adapts to new ones.  Every kernel of a call computes the same plan from the same numbers.
+// Work.  The new rows of a sequence and the G query heads of a key head are one list of n * G rows (row r: new token
+// r / G, head r % G of the group), cut into tiles; a tile has as many key steps (64 keys) as its sequence's rows see.  With
+// splits, the steps of all tiles of a key head stand in one line and each of its `parts` workgroups takes an equal piece of it,
+// wherever tiles begin and end: the lengths are known on the device only, and however unequal they are (and whatever a
+// recorded call meets when it is replayed) all workgroups end together.  A piece that is not a whole tile leaves an
+// unnormalised result, which join_kernel puts together.  Without splits a workgroup takes whole tiles.
+// Every kernel of a call computes the same plan from the same numbers.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kKeyStep = 64;  // splits begin and end at multiples of this many keys
+constexpr int kKeyStep = 64;
 
 struct Plan {
     int rows;       // rows of a tile
     int lo, hi;     // sequences with lo <= n * G <= hi belong to this kernel
-    int max_tiles;  // the grid and the workspace are made for this many tiles (of one key head) ...
-    int units;      // ... and units; more of either (a wrong hint): no splits
-    int per_head;   // workgroups worth having per key head
-    int min_steps;  // shortest split, in key steps
-    float* o;       // partial results [unit * Hkv + head][rows][D], unnormalised
+    int parts;      // workgroups per key head that share the steps; 0: no splits
+    int min_steps;  // fewest steps worth a workgroup
+    float* o;       // partial results [2 * part + (not the part's first piece)][Hkv][rows][D], unnormalised
     float* ml;      // [..][rows][2]: maximum (base 2, scaled) and sum
 };
 
 struct Share {  // what one sequence brings
-    int tiles, first, steps;  // row tiles; first key step its rows see; number of key steps
+    int tiles, first, steps;  // row tiles; first key step its rows see; number of steps of a tile
 };
 __device__ __forceinline__ Share share_of(const AttnArgs& a, const Plan& p, int s) {
     if (s >= a.g.S) return {0, 0, 0};
     const Seq q = seq_of(a.g, s);
     const int64_t rows = (int64_t)q.n * a.G;
     if (rows < 1 || rows < p.lo || rows > p.hi) return {0, 0, 0};
-    const Range r0 = visible(a, q, 0);
     const int hi = visible(a, q, q.n - 1).hi;
     Share x;
     x.tiles = (int)((rows + p.rows - 1) / p.rows);
-    x.first = r0.lo / kKeyStep;
-    x.steps = max(0, (hi + kKeyStep - 1) / kKeyStep - x.first);
+    x.first = visible(a, q, 0).lo / kKeyStep;
+    x.steps = max(1, (hi + kKeyStep - 1) / kKeyStep - x.first);  // (a tile that sees nothing is still stored)
     return x;
 }
+__device__ __forceinline__ int64_t weight_of(const Plan& p, const Share& x) {
+    return p.parts ? (int64_t)x.tiles * x.steps : x.tiles;
+}
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
+__device__ __forceinline__ int64_t lane64(int64_t x, int from) {  // (from: the same in every lane)
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, from);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), from);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t scan64(int64_t x, int lane) {  // sum over the lanes up to this one
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t lo = __shfl_xor((uint32_t)x, o, 64), hi = __shfl_xor((uint32_t)(x >> 32), o, 64);
-        x += (int64_t)(((uint64_t)hi << 32) | lo);
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t lo = __shfl_up((uint32_t)x, o, 64), hi = __shfl_up((uint32_t)(x >> 32), o, 64);
+        if (lane >= o) x += (int64_t)(((uint64_t)hi << 32) | lo);
     }
     return x;
 }
 
-// Key steps per split of this call (0x7fffffff: no splits), the same in every wave.
-__device__ __forceinline__ int split_steps(const AttnArgs& a, const Plan& p, int lane) {
-    int64_t work = 0, tiles = 0;
-    for (int base = 0; base < a.g.S; base += kWave) {
-        const Share x = share_of(a, p, base + lane);
-        work += (int64_t)x.tiles * x.steps;
-        tiles += x.tiles;
-    }
-    work = wave_sum64(work);
-    tiles = wave_sum64(tiles);
-    if (tiles > p.max_tiles || p.per_head < 1) return 0x7fffffff;
-    const int64_t per = (work + p.per_head - 1) / p.per_head;
-    // sum over tiles of ceil(steps / per) <= work / per + tiles <= per_head + max_tiles = units
-    return (int)max((int64_t)p.min_steps, per < 0x7fffffff ? per : 0x7fffffff);
-}
-__device__ __forceinline__ int splits_of(const Share& x, int per) {
-    return x.steps <= per ? 1 : (x.steps + per - 1) / per;
-}
-
-struct Unit {
-    int s, tile, split, n_splits, slot;  // slot: number of the unit (its place in the workspace)
-    int first, steps;                    // the sequence's key steps
+struct Piece {
+    int s, tile;      // sequence (-1: none), row tile
+    int first, steps; // key steps of the whole tile
+    int from;         // of them, where the position lies
 };
-// unit x of the call, s = -1 if there is none
-__device__ __forceinline__ Unit find_unit(const AttnArgs& a, const Plan& p, int per, int64_t x, int lane) {
-    Unit u;
-    u.s = -1;
-    int64_t before = 0;
-    for (int base = 0; base < a.g.S; base += kWave) {
-        const Share h = share_of(a, p, base + lane);
-        const int n_splits = splits_of(h, per);
-        // (tiles * splits of one sequence fits 32 bits: with splits there are at most `units` of them, without it is the
-        // number of tiles)
-        const int mine = h.tiles * n_splits;
-        int64_t sum = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t lo = __shfl_up((uint32_t)sum, o, 64), hi = __shfl_up((uint32_t)(sum >> 32), o, 64);
-            if (lane >= o) sum += (int64_t)(((uint64_t)hi << 32) | lo);
-        }
-        const bool here = x < before + sum;
-        const uint64_t vote = __builtin_amdgcn_ballot_w64(here);
-        if (vote) {
-            const int at = __builtin_ctzll(vote);
-            const int64_t start = before + sum - mine;
-            const int64_t rest = x - start;
-            u.s = base + at;
-            const int local = __shfl((int)rest, at, 64);
-            u.n_splits = __shfl(n_splits, at, 64);
-            u.first = __shfl(h.first, at, 64);
-            u.steps = __shfl(h.steps, at, 64);
-            u.tile = local / u.n_splits;
-            u.split = local % u.n_splits;
-            u.slot = (int)x;
-            return u;
-        }
-        before += wave_sum64(mine);
+
+// The line of work of one key head, held by a wave.
+struct Line {
+    Share mine;       // of sequence `lane`: batches of up to 64 sequences are read once
+    int64_t sum;      // weights of the sequences up to and with that one
+    int64_t total;
+    int parts;        // workgroups that share it (at most p.parts)
+
+    __device__ __forceinline__ void init(const AttnArgs& a, const Plan& p, int lane) {
+        mine = share_of(a, p, lane);
+        sum = scan64(weight_of(p, mine), lane);
+        total = lane64(sum, 63);
+        for (int base = kWave; base < a.g.S; base += kWave)
+            total += lane64(scan64(weight_of(p, share_of(a, p, base + lane)), lane), 63);
+        parts = 0;
+        if (p.parts) parts = (int)max((int64_t)1, min((int64_t)p.parts, total / p.min_steps));
     }
-    return u;
-}
-// keys [first, last) of a split: the steps are dealt out evenly
-__device__ __forceinline__ Range split_keys(const Unit& u) {
-    const int a = (int)((int64_t)u.steps * u.split / u.n_splits), b = (int)((int64_t)u.steps * (u.split + 1) / u.n_splits);
-    return {(u.first + a) * kKeyStep, (u.first + b) * kKeyStep};
-}
+    __device__ __forceinline__ int64_t start(int i) const { return total * i / parts; }            // of part i
+    __device__ __forceinline__ int part_of(int64_t x) const { return (int)(((x + 1) * parts - 1) / total); }
+
+    __device__ __forceinline__ Piece find(const AttnArgs& a, const Plan& p, int64_t x, int lane) const {
+        Piece r = {-1, 0, 0, 0, 0};
+        if (x >= total) return r;
+        Share h = mine;
+        int64_t upto = sum, before = 0;
+        for (int base = 0;;) {
+            const uint64_t vote = __builtin_amdgcn_ballot_w64(x < before + upto);
+            if (vote) {
+                const int at = __builtin_ctzll(vote);
+                const int64_t rest = x - lane64(before + upto - weight_of(p, h), at);
+                r.s = __builtin_amdgcn_readfirstlane(base + at);
+                r.first = __builtin_amdgcn_readlane(h.first, at);
+                r.steps = __builtin_amdgcn_readlane(h.steps, at);
+                r.tile = __builtin_amdgcn_readfirstlane((int)(p.parts ? rest / r.steps : rest));
+                r.from = __builtin_amdgcn_readfirstlane(p.parts ? (int)(rest - (int64_t)r.tile * r.steps) : 0);
+                return r;
+            }
+            before += lane64(upto, 63);
+            base += kWave;
+            h = share_of(a, p, base + lane);
+            upto = scan64(weight_of(p, h), lane);
+        }
+    }
+    // position of the first step of a sequence's first tile (s uniform)
+    __device__ __forceinline__ int64_t start_of(const AttnArgs& a, const Plan& p, int s, int lane) const {
+        Share h = mine;
+        int64_t upto = sum, before = 0;
+        for (int base = 0; s >= base + kWave;) {
+            before += lane64(upto, 63);
+            base += kWave;
+            h = share_of(a, p, base + lane);
+            upto = scan64(weight_of(p, h), lane);
+        }
+        return before + lane64(upto - weight_of(p, h), s & 63);
+    }
+};
 
 // Kernels that use more than 64 KB of LDS need the limit raised once per device: the one that owns the operands.
 template <auto kKernel>

@@ -19,27 +19,26 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan 
     if (s >= a.g.S) return;
     const Seq q = seq_of(a.g, s);
     if (row < q.q0 || row >= q.q0 + q.n) return;
-    const int per = split_steps(a, p, lane);
+    Line line;
+    line.init(a, p, lane);
     const Share mine = share_of(a, p, s);
-    const int n_splits = splits_of(mine, per);
-    if (mine.tiles == 0 || n_splits == 1) return;  // (one split: the unit has stored the result itself)
-    int64_t slot = 0;
-    for (int base = 0; base < s; base += kWave) {
-        const Share x = share_of(a, p, min(base + lane, s));
-        slot += wave_sum64(base + lane < s ? (int64_t)x.tiles * splits_of(x, per) : 0);
-    }
+    if (mine.tiles == 0) return;
     const int h = hq / a.G, r = (row - q.q0) * a.G + hq % a.G;
-    slot += (int64_t)(r / p.rows) * n_splits;
-    const int64_t first = (slot * a.Hkv + h) * p.rows + r % p.rows, step = (int64_t)a.Hkv * p.rows;
+    const int64_t from = line.start_of(a, p, s, lane) + (int64_t)(r / p.rows) * mine.steps;
+    const int i0 = line.part_of(from), i1 = line.part_of(from + mine.steps - 1);
+    if (i0 == i1) return;  // (one workgroup had the whole tile and has stored the result)
+    // the tile is the first piece of every part it reaches but perhaps the one it begins in
+    const int shift = from == line.start(i0) ? 0 : 1;
+    auto place = [&](int i) { return ((int64_t)(2 * i + (i == i0 ? shift : 0)) * a.Hkv + h) * p.rows + r % p.rows; };
     float top = -INFINITY;
-    for (int i = lane; i < n_splits; i += 64) top = fmaxf(top, p.ml[(first + i * step) * 2]);
+    for (int i = i0 + lane; i <= i1; i += 64) top = fmaxf(top, p.ml[place(i) * 2]);
     top = wave_max(top);
     float o[E], l = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
-    for (int i = wave; i < n_splits; i += kJoinWaves) {
-        const int64_t at = first + i * step;
+    for (int i = i0 + wave; i <= i1; i += kJoinWaves) {
+        const int64_t at = place(i);
         const float m = p.ml[at * 2];
         const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
         l += f * p.ml[at * 2 + 1];
@@ -65,18 +64,20 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan 
     store_row<Tag, D>(a, st, row, hq, lane);
 }
 
-// How a call is cut up (host side; the numbers of rows and keys themselves are known on the device only).
+// How a call is cut up (host side; how many rows and keys there are is known on the device only).
 struct Cut {
     Plan few;
     int64_t few_grid;
     size_t bytes;  // workspace
 };
 
-constexpr int kFewUnits = 512;  // workgroups that fill the chip: two per compute unit
+constexpr int kFewParts = 256;     // workgroups that fill the chip: one of 8 waves per compute unit
+constexpr int kWholeSteps = 32;    // a tile of so few key steps is not worth a split and the launch that joins it
 
 inline size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
 
-inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q) {
+// keys: most keys a row can see, as far as the caller's numbers tell
+inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t keys) {
     const int G = Hq / Hkv;
     Cut c{};
     const int64_t most = (int64_t)std::max(1, std::min(max_q, T)) * G;  // rows of a sequence
@@ -85,26 +86,30 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q) {
     p.lo = 1, p.hi = 0x7fffffff;
     const int64_t seqs = std::min(S, T);
     const int64_t tiles = std::min((int64_t)T * G / p.rows + seqs, seqs * ((most + p.rows - 1) / p.rows));
-    p.max_tiles = (int)std::min<int64_t>(tiles, 0x3fffffff);
-    p.per_head = tiles * Hkv >= kFewUnits ? 0 : (kFewUnits + Hkv - 1) / Hkv;
-    p.units = p.max_tiles + p.per_head;
-    p.min_steps = 4;
-    c.few_grid = (int64_t)p.units * Hkv;
-    if (p.per_head) {
-        const size_t rows = (size_t)p.units * Hkv * p.rows;
+    const bool whole = keys <= (int64_t)kWholeSteps * kKeyStep || tiles * Hkv >= 8 * kFewParts;
+    p.parts = whole ? 0 : std::max(1, kFewParts / Hkv);
+    p.min_steps = 8;
+    c.few_grid = (whole ? tiles : p.parts) * Hkv;
+    if (p.parts) {
+        const size_t rows = (size_t)2 * p.parts * Hkv * p.rows;
         c.bytes = round256(rows * D * 4) + round256(rows * 8);
     }
     return c;
 }
 
+inline int64_t most_keys(int width, int page, int causal, int window, int T, int max_q) {
+    const int64_t held = (int64_t)width * page;
+    return causal && window >= 0 ? std::min(held, (int64_t)window + std::max(1, std::min(max_q, T)) + kKeyStep) : held;
+}
+
 template <typename Tag>
 int run(AttnArgs& a, Cut& c, void* ws, int D, bool e4m3, hipStream_t stream) {
     Plan& p = c.few;
-    const size_t rows = (size_t)p.units * a.Hkv * p.rows;
+    const size_t rows = (size_t)2 * p.parts * a.Hkv * p.rows;
     p.o = (float*)ws;
     p.ml = (float*)((char*)ws + round256(rows * D * 4));
     if (int rc = launch_few<Tag>(a, p, D, e4m3, c.few_grid, stream)) return rc;
-    if (p.per_head) {
+    if (p.parts) {
         const dim3 grid((unsigned)((int64_t)a.g.T * a.Hq));
         if (D == 128)
             join_kernel<Tag, 128><<<grid, kJoinWaves * 64, 0, stream>>>(a, p);
@@ -138,7 +143,7 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
     a.window = window < 0 ? 1 << 30 : std::min(window, 1 << 30);
     a.scale_log2e = scale * kLog2e;
     if (S == 0 || T == 0) return VQA_OK;
-    Cut c = cut_call(T, S, Hq, Hkv, D, max_q);
+    Cut c = cut_call(T, S, Hq, Hkv, D, max_q, most_keys(width, page, causal, window, T, max_q));
     if (c.few_grid > 0x7fffffff) return VQA_ERR_BAD_SHAPE;
     if (c.bytes && ws == nullptr) return VQA_ERR_NULL_POINTER;
     if (reinterpret_cast<uintptr_t>(ws) % 256) return VQA_ERR_MISALIGNED;
@@ -151,9 +156,10 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
 
 extern "C" {
 
-size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int max_q) {
-    if (T < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || (D != 64 && D != 128)) return 0;
-    return vqa::paged::cut_call(T, S, Hq, Hkv, D, max_q).bytes;
+size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int page, int width, int causal, int window,
+                                      int max_q) {
+    if (T < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || page < 1 || width < 1) return 0;
+    return vqa::paged::cut_call(T, S, Hq, Hkv, D, max_q, vqa::paged::most_keys(width, page, causal, window, T, max_q)).bytes;
 }
 
 #define VQA_PAGED_ATTN(sfx, tag)                                                                                          \

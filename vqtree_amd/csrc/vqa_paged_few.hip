@@ -2,7 +2,7 @@
 // row of a (sequence, key head) is read once for all rows of a tile, 16 * NB of them (grouped query heads and new tokens
 // together).
 //
-// One workgroup is one unit (tile, split); its 4 waves take consecutive quarters of the split's keys and never wait for
+// One workgroup works on one piece of a tile's keys at a time; its waves take consecutive parts of it and never wait for
 // each other until their results are joined at the end.  A wave walks 32-key tiles: the rows go HBM -> LDS directly
 // (global_load_lds_dwordx4, whole rows per instruction, no registers), S^T = K.Q^T and O^T = V^T.P^T run on
 // v_mfma_f32_16x16x32 -- the matrix pipe has room to spare at any memory rate, so a single query row goes through it too.
@@ -17,7 +17,7 @@
 // are widened without factor, always to bf16 (exact), and the factor of the key goes to the probability instead, since a lane
 // then holds 8 keys of one d.  With f16 queries the scaled probability is split into two bf16 numbers (16 bits together), so
 // that neither f16's range nor bf16's 8 bits limit it.
-#include "vqa_flash.h"
+#include "vqa_flash2.h"
 #include "vqa_paged_attn.h"
 
 namespace vqa {
@@ -28,7 +28,7 @@ using flash::u32x4_t;
 typedef flash::s16x4_t s16x4_t;
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 constexpr int kKeys = 32;    // keys per tile
 constexpr float kLazy = 8.f; // a row's reference maximum moves when a tile exceeds it by 2^kLazy
 
@@ -77,79 +77,113 @@ __device__ __forceinline__ float quads_sum(float x) {
     return x + __shfl_xor(x, 32, 64);
 }
 
-// What a wave needs to bring a tile.
+// Brings tiles of one wave.
 template <int D, bool kE4m3>
 struct Loader {
     typedef Geo<D, kE4m3> G;
-    const AttnArgs* a;
-    const int32_t* table;   // of the sequence
-    int h, lane, end;       // keys from `end` on are not there
-    int row16, piece;       // this lane's row within 16 and LDS piece
-    int tab, tab0;          // table entries tab0 + lane
-    uint32_t lds;           // of the wave
+    const char *k, *v;             // pools at the key head
+    const uint8_t *ke, *ve;
+    const int32_t* table;          // of the sequence
+    int end;                       // keys from here on are not there
+    int lane;
+    int tab, tab0;                 // table entries tab0 + lane
+    uint32_t lds;                  // of the wave
+    uint32_t k_off[G::kLoads], v_off[G::kLoads];  // this lane's byte in a whole group of rows, per load
 
-    __device__ __forceinline__ void init(const AttnArgs& a_, int s, int h_, int end_, uint32_t lds_, int lane_) {
-        a = &a_;
-        table = a_.g.table + (int64_t)s * a_.g.table_ss;
-        h = h_, end = end_, lds = lds_, lane = lane_;
-        row16 = lane / G::kChunks;
-        piece = lane % G::kChunks;
+    static __device__ __forceinline__ int row_of_load(int i, int lane) { return (i * G::kRowsPerLoad) % 16 + lane / G::kChunks; }
+    template <bool kV>
+    static __device__ __forceinline__ uint32_t piece_of(int i, int lane) {
+        const int full = i * G::kRowsPerLoad + lane / G::kChunks;
+        return (uint32_t)((lane % G::kChunks) ^ (kV ? G::swz_v(full) : G::swz_k(full))) * 16u;
+    }
+    __device__ __forceinline__ void init(const AttnArgs& a, int h, uint32_t lds_, int lane_) {
+        k = a.kp.p + h * a.kp.sh, v = a.vp.p + h * a.vp.sh;
+        if constexpr (kE4m3) ke = a.kp.e + h * a.kp.eh, ve = a.vp.e + h * a.vp.eh;
+        lds = lds_, lane = lane_;
+#pragma unroll
+        for (int i = 0; i < G::kLoads; ++i) {
+            k_off[i] = (uint32_t)row_of_load(i, lane) * (uint32_t)a.kp.sn + piece_of<false>(i, lane);
+            v_off[i] = (uint32_t)row_of_load(i, lane) * (uint32_t)a.vp.sn + piece_of<true>(i, lane);
+        }
+    }
+    __device__ __forceinline__ void sequence(const AttnArgs& a, int s, int end_) {
+        table = a.g.table + (int64_t)s * a.g.table_ss;
+        end = end_;
         tab0 = -0x40000000;
         tab = -1;
     }
     // page of key j (below the table's end), -1 if it is not there
-    __device__ __forceinline__ int page_at(int j) {
-        const int c = j >> a->g.page_shift;
+    __device__ __forceinline__ int page_at(const Seqs& g, int j) {
+        const int c = j >> g.page_shift;
         if (c - tab0 >= 64 || c < tab0) {  // (uniform)
             tab0 = c;
-            tab = c + lane < a->g.width ? table[c + lane] : -1;
-            if ((unsigned)tab >= (unsigned)a->g.n_pages) tab = -1;
+            tab = c + lane < g.width ? table[c + lane] : -1;
+            if ((unsigned)tab >= (unsigned)g.n_pages) tab = -1;
         }
         return __builtin_amdgcn_readlane(tab, c - tab0);
     }
-    // Requests tile [j0, j0 + 32); the rows past `end` repeat the last one, pages that are not there read page 0 (their keys
-    // are hidden).  Returns which of its two 16-row groups are there.  kWhat: 1 keys (and exponents), 2 values.
-    template <int kWhat>
-    __device__ __forceinline__ int request(int j0, int slot) {
-        const uint32_t dst = lds + (uint32_t)(slot * G::kSlot) + (kWhat == 2 ? G::kTile : 0);
-        const Pool& pool = kWhat == 2 ? a->vp : a->kp;
-        int there = 0;
-        const char* group[2];
-        int last[2], page[2];
+    // Where the two 16-row groups of tile [j0, j0 + 32) lie.  Rows from `end` on repeat the last one that is there; a page
+    // that is not there reads page 0 (its keys are hidden).
+    struct Place {
+        int page[2], j[2];
+        int there;  // a bit per group
+    };
+    __device__ __forceinline__ Place place(const Seqs& g, int j0) {
+        Place x;
+        x.there = 0;
 #pragma unroll
         for (int gi = 0; gi < 2; ++gi) {
-            const int j = j0 + 16 * gi < end ? j0 + 16 * gi : (end - 1) & ~15;
-            const int p = page_at(j);
-            there |= p >= 0 ? 1 << gi : 0;
-            page[gi] = max(p, 0);
-            group[gi] = row_of(pool, a->g, page[gi], h, j);
-            last[gi] = min(15, end - 1 - j);
+            x.j[gi] = j0 + 16 * gi < end ? j0 + 16 * gi : (end - 1) & ~15;
+            const int p = page_at(g, x.j[gi]);
+            x.there |= p >= 0 ? 1 << gi : 0;
+            x.page[gi] = max(p, 0);
         }
+        return x;
+    }
+    template <bool kV>
+    __device__ __forceinline__ void request(const AttnArgs& a, const Place& x, int slot) {
+        const uint32_t dst = lds + (uint32_t)(slot * G::kSlot) + (kV ? G::kTile : 0);
+        const Pool& pool = kV ? a.vp : a.kp;
+        const int in_page = (1 << a.g.page_shift) - 1;
+        const char* group[2];
 #pragma unroll
-        for (int i = 0; i < G::kLoads; ++i) {
-            constexpr int kR = G::kRowsPerLoad;
-            const int gi = i * kR / 16;
-            const int r = (i * kR) % 16 + row16;  // row within the group
-            const int full = gi * 16 + r;
-            const int src = piece ^ (kWhat == 2 ? G::swz_v(full) : G::swz_k(full));
-            const uint32_t off = (uint32_t)min(r, last[gi]) * (uint32_t)pool.sn + (uint32_t)src * 16u;
-            flash::dma16_uniform(group[gi], off, dst + (uint32_t)(i * 1024));
+        for (int gi = 0; gi < 2; ++gi)
+            group[gi] = (kV ? v : k) + (int64_t)x.page[gi] * pool.sp + (int64_t)(x.j[gi] & in_page) * pool.sn;
+        if (x.j[1] + 16 <= end && x.j[0] != x.j[1]) {
+            flash2::static_for<G::kLoads>([&](auto I) {
+                constexpr int i = decltype(I)::value;
+                issue<i>(dst, kV ? v_off[i] : k_off[i], group[i * G::kRowsPerLoad / 16]);
+            });
+        } else {
+            flash2::static_for<G::kLoads>([&](auto I) {
+                constexpr int i = decltype(I)::value;
+                constexpr int gi = i * G::kRowsPerLoad / 16;
+                const uint32_t row = (uint32_t)min(row_of_load(i, lane), end - 1 - x.j[gi]);
+                issue<i>(dst, row * (uint32_t)pool.sn + piece_of<kV>(i, lane), group[gi]);
+            });
         }
-        if constexpr (kE4m3 && kWhat == 1) {
+        if constexpr (kE4m3 && !kV) {
             // lanes 0, 1: exponents of the two groups' keys, 2, 3: of their values
             if (lane < 4) {
-                const Pool& pe = lane < 2 ? a->kp : a->vp;
-                const int gi = lane & 1;
-                const int j = j0 + 16 * gi < end ? j0 + 16 * gi : (end - 1) & ~15;
-                flash::dma16(exp_of(pe, a->g, gi ? page[1] : page[0], h, j), lds + (uint32_t)(slot * G::kSlot + 2 * G::kTile));
+                const int64_t page = lane & 1 ? x.page[1] : x.page[0];
+                const int at = (lane & 1 ? x.j[1] : x.j[0]) & in_page;
+                flash::dma16((lane < 2 ? ke + page * a.kp.ep : ve + page * a.vp.ep) + at,
+                             lds + (uint32_t)(slot * G::kSlot + 2 * G::kTile));
             }
         }
-        return there;
+    }
+    template <int I>
+    static __device__ __forceinline__ void issue(uint32_t dst, uint32_t off, const char* base) {
+        // (a load may not follow the write of M0 directly)
+        asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
+                     :
+                     : "s"(dst), "n"(I * 1024), "v"(off), "s"(base)
+                     : "memory", "scc");
     }
 };
 
 template <typename Tag, int D, bool kE4m3, int NB>
-__global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(AttnArgs a, Plan p) {
+__global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
     typedef Geo<D, kE4m3> G;
     typedef typename Elem<Tag>::vec8 vec8;
     typedef typename std::conditional<kE4m3, bf16_tag, Tag>::type PTag;  // element type of the P.V product
@@ -169,32 +203,39 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(AttnArgs a, Plan p)
     const int n = lane & 15, quad = lane >> 4;
     const int h = __builtin_amdgcn_readfirstlane((int)(blockIdx.x % (unsigned)a.Hkv));
     const uint32_t lds0 = flash::lds_addr_of(smem);
-    const int per = split_steps(a, p, lane);
+    const int me = (int)(blockIdx.x / (unsigned)a.Hkv), n_wgs = (int)(gridDim.x / (unsigned)a.Hkv);
 
-    for (int64_t x = blockIdx.x / (unsigned)a.Hkv;; x += gridDim.x / (unsigned)a.Hkv) {
-        Unit u = find_unit(a, p, per, x, lane);
-        if (u.s < 0) return;
-        u.s = __builtin_amdgcn_readfirstlane(u.s);
+    Line line;
+    line.init(a, p, lane);
+    if (p.parts && me >= line.parts) return;
+    Loader<D, kE4m3> ld;
+    ld.init(a, h, lds0 + (uint32_t)(wave * G::kWaveBytes), lane);
+
+    const int64_t begin = p.parts ? line.start(me) : me, end = p.parts ? line.start(me + 1) : line.total;
+    for (int64_t x = begin; x < end;) {
+        const Piece u = line.find(a, p, x, lane);
         const Seq q = seq_of(a.g, u.s);
         const int n_rows = min(kRows, q.n * a.G - u.tile * kRows);  // (a tile is of one sequence: fits 32 bits)
-        const Range keys = split_keys(u);
-        const int u_lo = __builtin_amdgcn_readfirstlane(keys.lo);
-        const int u_hi = __builtin_amdgcn_readfirstlane(min(keys.hi, q.keys));
-        // this wave's quarter, in tiles
+        const int n_steps = p.parts ? (int)min((int64_t)(u.steps - u.from), end - x) : u.steps;
+        const bool whole = n_steps == u.steps;
+        const int slot_out = 2 * me + (x == begin ? 0 : 1);
+        x += p.parts ? n_steps : n_wgs;
+        const int u_lo = (u.first + u.from) * kKeyStep;
+        const int u_hi = __builtin_amdgcn_readfirstlane((int)min((int64_t)(u.first + u.from + n_steps) * kKeyStep, (int64_t)q.keys));
+        // this wave's part, in tiles
         const int n_tiles = max(0, (u_hi - u_lo + kKeys - 1) / kKeys);
         const int t_lo = n_tiles * wave / kWaves, t_hi = n_tiles * (wave + 1) / kWaves;
 
-        Loader<D, kE4m3> ld;
-        ld.init(a, u.s, h, u_hi, lds0 + (uint32_t)(wave * G::kWaveBytes), lane);
-        uint32_t there_bits = 0;  // two bits per tile in flight
+        ld.sequence(a, u.s, u_hi);
+        typename Loader<D, kE4m3>::Place places[G::kRing];
         auto ask_k = [&](int t, int slot) __attribute__((always_inline)) {
-            const int there = ld.template request<1>(u_lo + t * kKeys, slot);
-            there_bits = (there_bits & ~(3u << (2 * slot))) | ((uint32_t)there << (2 * slot));
+            places[slot] = ld.place(a.g, u_lo + t * kKeys);
+            ld.template request<false>(a, places[slot], slot);
         };
-        auto ask_v = [&](int t, int slot) __attribute__((always_inline)) { ld.template request<2>(u_lo + t * kKeys, slot); };
+        auto ask_v = [&](int slot) __attribute__((always_inline)) { ld.template request<true>(a, places[slot], slot); };
 #pragma unroll
         for (int i = 0; i < G::kRing; ++i)
-            if (t_lo + i < t_hi) ask_k(t_lo + i, i), ask_v(t_lo + i, i);
+            if (t_lo + i < t_hi) ask_k(t_lo + i, i), ask_v(i);
 
         // rows of this lane's columns: what they see, and their queries (rows past the end repeat the last)
         int lo[NB], hi[NB];
@@ -272,11 +313,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(AttnArgs a, Plan p)
                 const i32x2_t e = *(lds8_ptr)(uintptr_t)(base + 2 * G::kTile + 32 + quad * 8);
                 vexp[0] = (uint32_t)e[0], vexp[1] = (uint32_t)e[1];
             }
-            const uint32_t there = (there_bits >> (2 * slot)) & 3u;
+            const int there = places[slot].there;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile's keys are in registers: the slot may be refilled
             if (full) ask_k(t + G::kRing, slot);
 
-            const bool plain = j0 >= all_lo && j0 + kKeys <= all_hi && there == 3u;  // (uniform)
+            const bool plain = j0 >= all_lo && j0 + kKeys <= all_hi && there == 3;  // (uniform)
             if (!plain) {
                 const bool mine = (there >> (quad >> 1)) & 1;  // keys 8 * quad .. + 7 lie in one group of 16
 #pragma unroll
@@ -359,7 +400,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(AttnArgs a, Plan p)
                 }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (full) ask_v(t + G::kRing, slot);
+            if (full) ask_v(slot);
         };
         for (int t = t_lo; t < t_hi; t += G::kRing) {
 #pragma unroll
@@ -396,7 +437,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(AttnArgs a, Plan p)
         }
         __syncthreads();
         constexpr int kLanes = D / 8;  // threads per row, 8 elements each
-        const int64_t part = ((int64_t)u.slot * a.Hkv + h) * kRows;
+        const int64_t part = ((int64_t)slot_out * a.Hkv + h) * kRows;
 #pragma unroll
         for (int i = 0; i < kRows * kLanes / (kWaves * 64) + (kRows * kLanes % (kWaves * 64) ? 1 : 0); ++i) {
             const int at = i * kWaves * 64 + (int)threadIdx.x;
@@ -417,7 +458,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(AttnArgs a, Plan p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) probe += v[e] * 0.f;
             if (!(probe < INFINITY)) atomicOr(bad + r / 32, 1u << (r % 32));
-            if (u.n_splits > 1) {
+            if (!whole) {
                 float* dst = p.o + (part + r) * D + c * 8;
                 reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
                 reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -445,7 +486,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(AttnArgs a, Plan p)
             RowState<D> st;
             row_by_lanes<Tag, D, kE4m3>(a, u.s, h, a.q + (int64_t)(q.q0 + t) * a.q_st + (int64_t)hq * a.q_sh, max(u_lo, v.lo),
                                         min(u_hi, v.hi), st, lane);
-            if (u.n_splits > 1) {
+            if (!whole) {
 #pragma unroll
                 for (int e = 0; e < D / 64; ++e) p.o[(part + r) * D + lane * (D / 64) + e] = st.o[e];
                 if (lane == 0) {
