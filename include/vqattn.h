@@ -566,8 +566,8 @@ int vqa_paged_attn_f16(const void* q, const void* k_pages, const void* v_pages, 
                         int D, int page, int n_pages, int width, int e4m3, const int64_t* strides, int causal, int window,
                         int max_q, float sm_scale, vqa_stream_t stream);
 
-size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int page, int width, int causal, int window,
-                                      int max_q);
+size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int page, int width, int e4m3, int causal,
+                                      int window, int max_q);
 
 #ifdef __cplusplus
 }

@@ -106,7 +106,7 @@ def test_c_entries_refuse_before_any_launch(lib):
 
     def attn(**kw):
         a = dict(ok, **kw)
-        need = lib.vqa_paged_attn_workspace_bytes(a["T"], a["S"], a["Hq"], a["Hkv"], a["D"], a["page"], a["width"], a["causal"],
+        need = lib.vqa_paged_attn_workspace_bytes(a["T"], a["S"], a["Hq"], a["Hkv"], a["D"], a["page"], a["width"], a["e4m3"], a["causal"],
                                                   a["window"], a["T"])
         ws = kw.get("ws", need)
         return lib.vqa_paged_attn_bf16(a["q"], 16, 16, a["exp"], a["exp"], 16, 16, 16, 16, None, 256, ws, a["T"], a["S"],

@@ -74,7 +74,7 @@ SIGNATURES = {
     "vqa_paged_read_f16": (c_int, [_P] * 8 + [c_int] * 8 + [_STRIDES, _P]),
     "vqa_paged_attn_bf16": (c_int, [_P] * 11 + [c_size_t] + [c_int] * 9 + [_STRIDES, c_int, c_int, c_int, c_float, _P]),
     "vqa_paged_attn_f16": (c_int, [_P] * 11 + [c_size_t] + [c_int] * 9 + [_STRIDES, c_int, c_int, c_int, c_float, _P]),
-    "vqa_paged_attn_workspace_bytes": (c_size_t, [c_int] * 10),
+    "vqa_paged_attn_workspace_bytes": (c_size_t, [c_int] * 11),
 }
 
 

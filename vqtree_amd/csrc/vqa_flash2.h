@@ -155,6 +155,7 @@ struct Wave {
     float l[2][2];                 // two partial row sums per block (even / odd keys of the lane)
     u32x4_t p[2][4];               // packed probabilities of the current tile: [block][16-key step]
     float ex[2][2];                // exp stream: exponentials of the current unit and of the one before
+    float c;                       // Pipe<..., kRaw = true> only: scale * log2(e), applied to every score
 
     __device__ __forceinline__ void init() {
 #pragma unroll
@@ -226,7 +227,10 @@ struct TileDma {
     }
 };
 
-template <typename Tag, int D, int NW = 4>
+// kRaw: the query is NOT pre-multiplied; scores and maxima are in units of q.k and the exponent takes a multiplication per
+// score (two more micro-ops per unit).  For callers whose log-sum-exp has to be accurate to fp32: the pre-multiplied query
+// carries a rounding of its own.
+template <typename Tag, int D, int NW = 4, bool kRaw = false>
 struct Pipe {
     typedef Geom<D> G;
     typedef typename Elem<Tag>::vec8 vec8;
@@ -243,12 +247,13 @@ struct Pipe {
     //   exp stream of the CURRENT tile: 5 micro-ops per stream step, kUnits + 1 steps (see exp_micro_op); the first
     //   kMicroScore of them run under the score MFMAs of the NEXT tile, the rest under the first kPvStream P.V MFMAs;
     //   row maxima of the NEXT tile: kUnits v_max3 over the P.V slots from kMaxFirst on.
-    static constexpr int kMicroOps = 5 * (kUnits + 1);
+    static constexpr int kStep = kRaw ? 7 : 5;  // micro-ops per stream step
+    static constexpr int kMicroOps = kStep * (kUnits + 1);
 #ifdef VQA_TUNE_MICRO_SCORE
     static constexpr int kMicroScore = VQA_TUNE_MICRO_SCORE;
     static constexpr int kPvStream = VQA_TUNE_PV_STREAM;
 #else
-    static constexpr int kMicroScore = D == 128 ? 100 : 80;
+    static constexpr int kMicroScore = (D == 128 ? 20 : 16) * kStep;
     static constexpr int kPvStream = D == 128 ? 22 : 11;
 #endif
 #ifdef VQA_TUNE_MAX_FIRST
@@ -272,7 +277,7 @@ struct Pipe {
     // a slot to spare, before the first P.V MFMA that reads them
     static constexpr bool deadlines_met() {
         for (int j = 0; j < 4; ++j)
-            if (micro_done(kScoreSlots + 2 * DB * j - 2) < 5 * (8 * j + 8) + 3) return false;
+            if (micro_done(kScoreSlots + 2 * DB * j - 2) < kStep * (8 * j + 8) + kStep - 2) return false;
         return true;
     }
     static_assert(deadlines_met(), "the exp stream is too late for the P.V products");
@@ -315,12 +320,19 @@ struct Pipe {
     // of that pipe (measured: MFMA + 4 v_dot2c 69 clocks, MFMA + 4 of any other VALU instruction 39).
     template <int X>
     static __device__ __forceinline__ void exp_micro_op(Wave<Tag, D>& w, const Scores& sc) {
-        constexpr int K = X / 5, part = X % 5;
-        if constexpr (part < 2) {
+        constexpr int K = X / kStep, part = X % kStep - (kRaw ? 2 : 0);
+        if constexpr (part < 0) {
             if constexpr (K < kUnits) {
                 constexpr int step = K / 8, qb = (K / 4) % 2, e = K % 4;
                 constexpr int kb = step / 2, j2 = step % 2, r = j2 * 8 + 2 * e;
-                w.ex[K % 2][part] = fast_exp2(sc.s[qb][kb][r + part]);
+                w.ex[K % 2][part + 2] = sc.s[qb][kb][r + part + 2] * w.c;
+                pin(w.ex[K % 2][part + 2]);
+            }
+        } else if constexpr (part < 2) {
+            if constexpr (K < kUnits) {
+                constexpr int step = K / 8, qb = (K / 4) % 2, e = K % 4;
+                constexpr int kb = step / 2, j2 = step % 2, r = j2 * 8 + 2 * e;
+                w.ex[K % 2][part] = fast_exp2(kRaw ? w.ex[K % 2][part] : sc.s[qb][kb][r + part]);
                 pin(w.ex[K % 2][part]);
             }
         } else if constexpr (K >= 1) {
@@ -474,8 +486,9 @@ struct Pipe {
     // The usual case -- no row of the wave moves -- is two compares and a branch: a row's maximum is the larger of the
     // values its two lanes hold, so "some row exceeds its threshold" can be read off the lanes before they are joined.
     static __device__ __forceinline__ void update_max(Wave<Tag, D>& w, const float (&mx)[2], Scores& sc) {
-        const bool any0 = mx[0] > ((w.m[0] == -INFINITY) ? -INFINITY : kLazy);
-        const bool any1 = mx[1] > ((w.m[1] == -INFINITY) ? -INFINITY : kLazy);
+        const float lazy = kRaw ? kLazy / w.c : kLazy;
+        const bool any0 = mx[0] > ((w.m[0] == -INFINITY) ? -INFINITY : lazy);
+        const bool any1 = mx[1] > ((w.m[1] == -INFINITY) ? -INFINITY : lazy);
         if (__builtin_amdgcn_ballot_w64(any0 || any1) == 0) return;
         // rows that see their first key have l = O = 0: nothing to rescale.  That is every row at the start of a query
         // tile, so the first tile of a key loop does not pay for reading and writing all of O.
@@ -486,11 +499,11 @@ struct Pipe {
         for (int qb = 0; qb < 2; ++qb) {
             const float rel = join_halves_max(mx[qb]);
             const bool first = w.m[qb] == -INFINITY;
-            const bool need = rel > (first ? -INFINITY : kLazy);
+            const bool need = rel > (first ? -INFINITY : lazy);
             const float delta = need ? rel : 0.f;
             if (rescale) {
                 // (a first key among rows that do move: any finite factor keeps l = O = 0; 2^-rel may overflow)
-                const float alpha = (need && !first) ? fast_exp2(-delta) : (need ? 0.f : 1.f);
+                const float alpha = (need && !first) ? fast_exp2(kRaw ? -delta * w.c : -delta) : (need ? 0.f : 1.f);
                 w.l[qb][0] *= alpha;
                 w.l[qb][1] *= alpha;
 #pragma unroll

@@ -145,12 +145,12 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& 
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Work.  The new rows of a sequence and the G query heads of a key head are one list of n * G rows (row r: new token
-// r / G, head r % G of the group), cut into tiles; a tile has as many key steps (64 keys) as its sequence's rows see.  With
-// splits, the steps of all tiles of a key head stand in one line and each of its `parts` workgroups takes an equal piece of it,
-// wherever tiles begin and end: the lengths are known on the device only, and however unequal they are (and whatever a
-// recorded call meets when it is replayed) all workgroups end together.  A piece that is not a whole tile leaves an
-// unnormalised result, which join_kernel puts together.  Without splits a workgroup takes whole tiles.
-// Every kernel of a call computes the same plan from the same numbers.
+// r / G, head r % G of the group), cut into tiles; a tile has as many key steps (64 keys) as its rows see.  With splits, the
+// steps of all tiles of a key head stand in one line and each of its `parts` workgroups takes an equal piece of it, wherever
+// tiles begin and end: the lengths are known on the device only, and however unequal they are (and whatever a recorded call
+// meets when it is replayed) all workgroups end together.  A piece that is not a whole tile leaves an unnormalised result,
+// which join_kernel puts together.  Without splits a workgroup takes whole tiles, the last (longest) ones of the sequences
+// first.  Every kernel of a call computes the same plan from the same numbers.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kKeyStep = 64;
 
@@ -163,23 +163,15 @@ struct Plan {
     float* ml;      // [..][rows][2]: maximum (base 2, scaled) and sum
 };
 
-struct Share {  // what one sequence brings
-    int tiles, first, steps;  // row tiles; first key step its rows see; number of steps of a tile
-};
-__device__ __forceinline__ Share share_of(const AttnArgs& a, const Plan& p, int s) {
-    if (s >= a.g.S) return {0, 0, 0};
-    const Seq q = seq_of(a.g, s);
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, const Plan& p, const Seq& q) {
     const int64_t rows = (int64_t)q.n * a.G;
-    if (rows < 1 || rows < p.lo || rows > p.hi) return {0, 0, 0};
-    const int hi = visible(a, q, q.n - 1).hi;
-    Share x;
-    x.tiles = (int)((rows + p.rows - 1) / p.rows);
-    x.first = visible(a, q, 0).lo / kKeyStep;
-    x.steps = max(1, (hi + kKeyStep - 1) / kKeyStep - x.first);  // (a tile that sees nothing is still stored)
-    return x;
+    return rows < 1 || rows < p.lo || rows > p.hi ? 0 : (int)((rows + p.rows - 1) / p.rows);
 }
-__device__ __forceinline__ int64_t weight_of(const Plan& p, const Share& x) {
-    return p.parts ? (int64_t)x.tiles * x.steps : x.tiles;
+// key steps [first, first + steps) of tile t; a tile that sees nothing has one (its result is still stored)
+__device__ __forceinline__ void steps_of(const AttnArgs& a, const Plan& p, const Seq& q, int t, int& first, int& steps) {
+    const int last_row = (int)min((int64_t)(t + 1) * p.rows, (int64_t)q.n * a.G) - 1;
+    first = visible(a, q, t * p.rows / a.G).lo / kKeyStep;
+    steps = max(1, (visible(a, q, last_row / a.G).hi + kKeyStep - 1) / kKeyStep - first);
 }
 
 __device__ __forceinline__ int64_t lane64(int64_t x, int from) {  // (from: the same in every lane)
@@ -187,7 +179,15 @@ __device__ __forceinline__ int64_t lane64(int64_t x, int from) {  // (from: the 
     const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), from);
     return (int64_t)(((uint64_t)hi << 32) | lo);
 }
-__device__ __forceinline__ int64_t scan64(int64_t x, int lane) {  // sum over the lanes up to this one
+__device__ __forceinline__ int scan32(int x, int lane) {  // sum over the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+__device__ __forceinline__ int64_t scan64(int64_t x, int lane) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const uint32_t lo = __shfl_up((uint32_t)x, o, 64), hi = __shfl_up((uint32_t)(x >> 32), o, 64);
@@ -197,66 +197,124 @@ __device__ __forceinline__ int64_t scan64(int64_t x, int lane) {  // sum over th
 }
 
 struct Piece {
-    int s, tile;      // sequence (-1: none), row tile
-    int first, steps; // key steps of the whole tile
-    int from;         // of them, where the position lies
+    int s, tile;       // sequence, row tile
+    Seq q;
+    int first, steps;  // key steps of the whole tile
+    int from;          // of them, where the position lies
 };
 
-// The line of work of one key head, held by a wave.
+// The line of one key head's tiles, held by a wave: 64 tiles at a time, one in each lane.
 struct Line {
-    Share mine;       // of sequence `lane`: batches of up to 64 sequences are read once
-    int64_t sum;      // weights of the sequences up to and with that one
-    int64_t total;
-    int parts;        // workgroups that share it (at most p.parts)
+    int base;             // number of lane 0's tile
+    int s, t;             // of this lane's tile: sequence, tile of the sequence
+    Seq q;
+    int first, steps;     // its key steps (steps 0: there is no such tile)
+    int64_t before, sum;  // steps before this block of tiles; in it, up to and with this lane's
+    int64_t total;        // steps (with splits) or tiles of the whole line
+    int n_tiles;
+    int parts;            // workgroups that share the line (at most p.parts)
 
-    __device__ __forceinline__ void init(const AttnArgs& a, const Plan& p, int lane) {
-        mine = share_of(a, p, lane);
-        sum = scan64(weight_of(p, mine), lane);
-        total = lane64(sum, 63);
-        for (int base = kWave; base < a.g.S; base += kWave)
-            total += lane64(scan64(weight_of(p, share_of(a, p, base + lane)), lane), 63);
-        parts = 0;
-        if (p.parts) parts = (int)max((int64_t)1, min((int64_t)p.parts, total / p.min_steps));
+    // Tiles base .. base + 63: each lane looks for its tile in the running count of tiles over the sequences.
+    __device__ __forceinline__ void block(const AttnArgs& a, const Plan& p, int base_, int lane) {
+        base = base_;
+        steps = 0, first = 0, s = 0, t = 0, q = Seq{0, 0, 0, 0};
+        int seen = 0;
+        for (int sb = 0; sb < a.g.S; sb += kWave) {
+            Seq x = {0, 0, 0, 0};
+            if (sb + lane < a.g.S) x = seq_of(a.g, sb + lane);
+            const int mine = tiles_of(a, p, x);
+            const int upto = scan32(mine, lane);
+            const int here = __builtin_amdgcn_readlane(upto, 63);
+            const int want = base + lane - seen;
+            if (base + kWave > seen && base < seen + here) {  // (uniform: some lane's tile is one of these sequences')
+                int at = 0;
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) at += __shfl(upto, at + o - 1, 64) <= want ? o : 0;
+                const int start = __shfl(upto - mine, at, 64);
+                const Seq y = {__shfl(x.q0, at, 64), __shfl(x.n, at, 64), __shfl(x.len, at, 64), __shfl(x.keys, at, 64)};
+                if (want >= 0 && want < here) {
+                    s = sb + at, t = want - start, q = y;
+                    steps_of(a, p, q, t, first, steps);
+                }
+            }
+            seen += here;
+        }
+        n_tiles = seen;
+        sum = scan64(p.parts ? steps : (steps > 0 ? 1 : 0), lane);
     }
-    __device__ __forceinline__ int64_t start(int i) const { return total * i / parts; }            // of part i
+    __device__ __forceinline__ void init(const AttnArgs& a, const Plan& p, int lane) {
+        block(a, p, 0, lane);
+        before = 0;
+        total = lane64(sum, 63);
+        parts = 0;
+        if (!p.parts) {
+            total = n_tiles;
+            return;
+        }
+        if (n_tiles > kWave) {
+            for (int b = kWave; b < n_tiles; b += kWave) {
+                block(a, p, b, lane);
+                total += lane64(sum, 63);
+            }
+            block(a, p, 0, lane);
+        }
+        parts = (int)max((int64_t)1, min((int64_t)p.parts, total / p.min_steps));
+    }
+    __device__ __forceinline__ int64_t start(int i) const { return total * i / parts; }  // of part i
     __device__ __forceinline__ int part_of(int64_t x) const { return (int)(((x + 1) * parts - 1) / total); }
 
-    __device__ __forceinline__ Piece find(const AttnArgs& a, const Plan& p, int64_t x, int lane) const {
-        Piece r = {-1, 0, 0, 0, 0};
-        if (x >= total) return r;
-        Share h = mine;
-        int64_t upto = sum, before = 0;
-        for (int base = 0;;) {
-            const uint64_t vote = __builtin_amdgcn_ballot_w64(x < before + upto);
-            if (vote) {
-                const int at = __builtin_ctzll(vote);
-                const int64_t rest = x - lane64(before + upto - weight_of(p, h), at);
-                r.s = __builtin_amdgcn_readfirstlane(base + at);
-                r.first = __builtin_amdgcn_readlane(h.first, at);
-                r.steps = __builtin_amdgcn_readlane(h.steps, at);
-                r.tile = __builtin_amdgcn_readfirstlane((int)(p.parts ? rest / r.steps : rest));
-                r.from = __builtin_amdgcn_readfirstlane(p.parts ? (int)(rest - (int64_t)r.tile * r.steps) : 0);
-                return r;
-            }
-            before += lane64(upto, 63);
-            base += kWave;
-            h = share_of(a, p, base + lane);
-            upto = scan64(weight_of(p, h), lane);
+    // the tile at position x < total; positions of later calls do not decrease
+    __device__ __forceinline__ Piece find(const AttnArgs& a, const Plan& p, int64_t x, int lane) {
+        while (x >= before + lane64(sum, 63)) {
+            before += lane64(sum, 63);
+            block(a, p, base + kWave, lane);
         }
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(x < before + sum));
+        Piece r;
+        r.s = __builtin_amdgcn_readlane(s, at);
+        r.tile = __builtin_amdgcn_readlane(t, at);
+        r.q = Seq{__builtin_amdgcn_readlane(q.q0, at), __builtin_amdgcn_readlane(q.n, at),
+                  __builtin_amdgcn_readlane(q.len, at), __builtin_amdgcn_readlane(q.keys, at)};
+        r.first = __builtin_amdgcn_readlane(first, at);
+        r.steps = __builtin_amdgcn_readlane(steps, at);
+        r.from = p.parts ? (int)(x - before - lane64(sum - steps, at)) : 0;
+        return r;
     }
-    // position of the first step of a sequence's first tile (s uniform)
-    __device__ __forceinline__ int64_t start_of(const AttnArgs& a, const Plan& p, int s, int lane) const {
-        Share h = mine;
-        int64_t upto = sum, before = 0;
-        for (int base = 0; s >= base + kWave;) {
-            before += lane64(upto, 63);
-            base += kWave;
-            h = share_of(a, p, base + lane);
-            upto = scan64(weight_of(p, h), lane);
+    // position of tile number i < n_tiles, and its key steps
+    __device__ __forceinline__ int64_t start_of_tile(const AttnArgs& a, const Plan& p, int i, int& n_steps, int lane) {
+        while (i >= base + kWave) {
+            before += lane64(sum, 63);
+            block(a, p, base + kWave, lane);
         }
-        return before + lane64(upto - weight_of(p, h), s & 63);
+        n_steps = __builtin_amdgcn_readlane(steps, i - base);
+        return before + lane64(sum - steps, i - base);
     }
 };
+
+// What a workgroup does: calls work(piece, first step, steps, whole, place in the workspace) for each of its pieces.  (The
+// line's block is made again behind a piece, so that it takes no registers meanwhile.)
+template <typename F>
+__device__ __forceinline__ void for_each_piece(const AttnArgs& a, const Plan& p, int me, int n_wgs, int lane, F&& work) {
+    Line line;
+    line.init(a, p, lane);
+    if (p.parts && me >= line.parts) return;
+    const int64_t begin = p.parts ? line.start(me) : line.total - 1 - me;  // (whole tiles: the longest, last ones first)
+    const int64_t end = p.parts ? line.start(me + 1) : 0;
+    int64_t x = begin;
+    if (p.parts ? x >= end : x < 0) return;
+    for (;;) {
+        if (!p.parts && (x < line.base || x >= line.base + kWave)) {
+            line.before = x & ~(int64_t)(kWave - 1);
+            line.block(a, p, (int)line.before, lane);
+        }
+        const Piece u = line.find(a, p, x, lane);
+        const int n = p.parts ? (int)min((int64_t)(u.steps - u.from), end - x) : u.steps;
+        work(u, u.first + u.from, n, n == u.steps, 2 * me + (x == begin ? 0 : 1));
+        x += p.parts ? n : -n_wgs;
+        if (p.parts ? x >= end : x < 0) return;
+        line.block(a, p, line.base, lane);
+    }
+}
 
 // Kernels that use more than 64 KB of LDS need the limit raised once per device: the one that owns the operands.
 template <auto kKernel>
@@ -277,6 +335,8 @@ int raise_lds(const void* operand, int bytes) {
 
 template <typename Tag>
 int launch_few(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream);
+template <typename Tag>
+int launch_chunk(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream);
 
 }  // namespace paged
 }  // namespace vqa

@@ -11,7 +11,7 @@ namespace paged {
 constexpr int kJoinWaves = 4;
 
 template <typename Tag, int D>
-__global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan p) {
+__global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan few, Plan chunk) {
     constexpr int E = D / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = (int)(blockIdx.x / (unsigned)a.Hq), hq = (int)(blockIdx.x % (unsigned)a.Hq);
@@ -19,13 +19,19 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan 
     if (s >= a.g.S) return;
     const Seq q = seq_of(a.g, s);
     if (row < q.q0 || row >= q.q0 + q.n) return;
+    const Plan p = tiles_of(a, few, q) ? few : chunk;
+    if (p.parts == 0) return;  // (whole tiles)
     Line line;
     line.init(a, p, lane);
-    const Share mine = share_of(a, p, s);
-    if (mine.tiles == 0) return;
+    int tile = 0;  // number of the row's tile: the tiles of the sequences before it, then its own
+    for (int base = 0; base < s; base += kWave) {
+        const int mine = base + lane < s ? tiles_of(a, p, seq_of(a.g, base + lane)) : 0;
+        tile += __builtin_amdgcn_readlane(scan32(mine, lane), 63);
+    }
     const int h = hq / a.G, r = (row - q.q0) * a.G + hq % a.G;
-    const int64_t from = line.start_of(a, p, s, lane) + (int64_t)(r / p.rows) * mine.steps;
-    const int i0 = line.part_of(from), i1 = line.part_of(from + mine.steps - 1);
+    int n_steps;
+    const int64_t from = line.start_of_tile(a, p, tile + r / p.rows, n_steps, lane);
+    const int i0 = line.part_of(from), i1 = line.part_of(from + n_steps - 1);
     if (i0 == i1) return;  // (one workgroup had the whole tile and has stored the result)
     // the tile is the first piece of every part it reaches but perhaps the one it begins in
     const int shift = from == line.start(i0) ? 0 : 1;
@@ -66,34 +72,40 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan 
 
 // How a call is cut up (host side; how many rows and keys there are is known on the device only).
 struct Cut {
-    Plan few;
-    int64_t few_grid;
-    size_t bytes;  // workspace
+    Plan few, chunk;                // (a plan without rows: its kernel is not needed)
+    int64_t few_grid, chunk_grid;
+    size_t few_bytes, chunk_bytes;  // workspace
 };
 
-constexpr int kFewParts = 256;     // workgroups that fill the chip: one of 8 waves per compute unit
-constexpr int kWholeSteps = 32;    // a tile of so few key steps is not worth a split and the launch that joins it
+constexpr int kCus = 256;           // workgroups that fill the chip: one per compute unit, in both kernels
+constexpr int kWholeSteps = 32;     // a tile of so few key steps is not worth a split and the launch that joins it
+constexpr int kFewRows = 64;        // sequences of more rows go to the chunk kernel
 
 inline size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
+inline size_t o_bytes(const Plan& p, int Hkv, int D) { return round256((size_t)2 * p.parts * Hkv * p.rows * D * 4); }
+inline size_t ml_bytes(const Plan& p, int Hkv) { return round256((size_t)2 * p.parts * Hkv * p.rows * 8); }
 
 // keys: most keys a row can see, as far as the caller's numbers tell
-inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t keys) {
+inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t keys, bool e4m3) {
     const int G = Hq / Hkv;
     Cut c{};
     const int64_t most = (int64_t)std::max(1, std::min(max_q, T)) * G;  // rows of a sequence
-    Plan& p = c.few;
-    p.rows = most <= 16 ? 16 : 32;
-    p.lo = 1, p.hi = 0x7fffffff;
-    const int64_t seqs = std::min(S, T);
-    const int64_t tiles = std::min((int64_t)T * G / p.rows + seqs, seqs * ((most + p.rows - 1) / p.rows));
-    const bool whole = keys <= (int64_t)kWholeSteps * kKeyStep || tiles * Hkv >= 8 * kFewParts;
-    p.parts = whole ? 0 : std::max(1, kFewParts / Hkv);
-    p.min_steps = 8;
-    c.few_grid = (whole ? tiles : p.parts) * Hkv;
-    if (p.parts) {
-        const size_t rows = (size_t)2 * p.parts * Hkv * p.rows;
-        c.bytes = round256(rows * D * 4) + round256(rows * 8);
-    }
+    const int64_t seqs = std::min(S, T), all = (int64_t)T * G;
+    const int limit = !e4m3 && most > kFewRows ? kFewRows : 0x7fffffff;
+    const bool short_keys = keys <= (int64_t)kWholeSteps * kKeyStep;
+    auto plan = [&](int rows, int lo, int hi, int whole_from, int min_steps, Plan& p, int64_t& grid, size_t& bytes) {
+        const int64_t rows_each = std::min<int64_t>(most, hi);
+        const int64_t tiles = std::min(all / rows + seqs, seqs * ((rows_each + rows - 1) / rows));
+        p.rows = rows, p.lo = lo, p.hi = hi;
+        p.parts = tiles * Hkv >= whole_from || short_keys ? 0 : std::max(1, kCus / Hkv);
+        p.min_steps = min_steps;
+        grid = (p.parts ? p.parts : tiles) * Hkv;
+        bytes = p.parts ? o_bytes(p, Hkv, D) + ml_bytes(p, Hkv) : 0;
+    };
+    // (a hint that is too small keeps every sequence in the few-rows kernel; one that is too large costs an idle launch)
+    if (!(most > limit && S == 1 && max_q >= T && all > kFewRows))
+        plan(std::min<int64_t>(most, limit) <= 16 ? 16 : 32, 1, limit, 8 * kCus, 8, c.few, c.few_grid, c.few_bytes);
+    if (most > limit) plan(256, limit + 1, 0x7fffffff, 4 * kCus, 4, c.chunk, c.chunk_grid, c.chunk_bytes);
     return c;
 }
 
@@ -103,18 +115,24 @@ inline int64_t most_keys(int width, int page, int causal, int window, int T, int
 }
 
 template <typename Tag>
-int run(AttnArgs& a, Cut& c, void* ws, int D, bool e4m3, hipStream_t stream) {
-    Plan& p = c.few;
-    const size_t rows = (size_t)2 * p.parts * a.Hkv * p.rows;
-    p.o = (float*)ws;
-    p.ml = (float*)((char*)ws + round256(rows * D * 4));
-    if (int rc = launch_few<Tag>(a, p, D, e4m3, c.few_grid, stream)) return rc;
-    if (p.parts) {
+int run(const AttnArgs& a, Cut& c, void* ws, int D, bool e4m3, hipStream_t stream) {
+    char* at = (char*)ws;
+    for (Plan* p : {&c.few, &c.chunk}) {
+        p->o = (float*)at;
+        at += o_bytes(*p, a.Hkv, D);
+        p->ml = (float*)at;
+        at += ml_bytes(*p, a.Hkv);
+    }
+    if (c.chunk.rows)
+        if (int rc = launch_chunk<Tag>(a, c.chunk, D, e4m3, c.chunk_grid, stream)) return rc;
+    if (c.few.rows)
+        if (int rc = launch_few<Tag>(a, c.few, D, e4m3, c.few_grid, stream)) return rc;
+    if (c.few.parts || c.chunk.parts) {
         const dim3 grid((unsigned)((int64_t)a.g.T * a.Hq));
         if (D == 128)
-            join_kernel<Tag, 128><<<grid, kJoinWaves * 64, 0, stream>>>(a, p);
+            join_kernel<Tag, 128><<<grid, kJoinWaves * 64, 0, stream>>>(a, c.few, c.chunk);
         else
-            join_kernel<Tag, 64><<<grid, kJoinWaves * 64, 0, stream>>>(a, p);
+            join_kernel<Tag, 64><<<grid, kJoinWaves * 64, 0, stream>>>(a, c.few, c.chunk);
         return launch_status();
     }
     return VQA_OK;
@@ -143,11 +161,12 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
     a.window = window < 0 ? 1 << 30 : std::min(window, 1 << 30);
     a.scale_log2e = scale * kLog2e;
     if (S == 0 || T == 0) return VQA_OK;
-    Cut c = cut_call(T, S, Hq, Hkv, D, max_q, most_keys(width, page, causal, window, T, max_q));
-    if (c.few_grid > 0x7fffffff) return VQA_ERR_BAD_SHAPE;
-    if (c.bytes && ws == nullptr) return VQA_ERR_NULL_POINTER;
+    Cut c = cut_call(T, S, Hq, Hkv, D, max_q, most_keys(width, page, causal, window, T, max_q), e4m3 != 0);
+    if (c.few_grid > 0x7fffffff || c.chunk_grid > 0x7fffffff) return VQA_ERR_BAD_SHAPE;
+    const size_t bytes = c.few_bytes + c.chunk_bytes;
+    if (bytes && ws == nullptr) return VQA_ERR_NULL_POINTER;
     if (reinterpret_cast<uintptr_t>(ws) % 256) return VQA_ERR_MISALIGNED;
-    if (ws_bytes < c.bytes) return VQA_ERR_WORKSPACE_TOO_SMALL;
+    if (ws_bytes < bytes) return VQA_ERR_WORKSPACE_TOO_SMALL;
     return run<Tag>(a, c, ws, D, e4m3 != 0, stream);
 }
 
@@ -156,10 +175,12 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
 
 extern "C" {
 
-size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int page, int width, int causal, int window,
-                                      int max_q) {
+size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int page, int width, int e4m3, int causal,
+                                      int window, int max_q) {
     if (T < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || page < 1 || width < 1) return 0;
-    return vqa::paged::cut_call(T, S, Hq, Hkv, D, max_q, vqa::paged::most_keys(width, page, causal, window, T, max_q)).bytes;
+    const vqa::paged::Cut c = vqa::paged::cut_call(
+        T, S, Hq, Hkv, D, max_q, vqa::paged::most_keys(width, page, causal, window, T, max_q), e4m3 != 0);
+    return c.few_bytes + c.chunk_bytes;
 }
 
 #define VQA_PAGED_ATTN(sfx, tag)                                                                                          \

@@ -1,0 +1,323 @@
+// Many rows: chunks of prompts (vqa_paged_attn_*), on the software-pipelined core of vqa_flash2.h.  MFMA bound.
+//
+// One workgroup of 4 waves owns a tile of 256 rows (grouped query heads and tokens together, so a chunk of 64 tokens with
+// 4 query heads per key head fills one) and walks 64-key tiles of the piece it was given; a wave brings 16 rows of each
+// tile, which lie in one page, so paging costs the key loop one look-up and two row addresses per tile, in scalar registers.
+// Rows of a tile differ in what they see; masks are evaluated per element only on tiles where they do (diagonal, window
+// edge, end, missing pages).
+//
+// kRaw (a call that asks for the log-sum-exp): scores are scaled in fp32 behind the product; otherwise the query is
+// pre-multiplied by scale * log2(e) and rounded once more, which saves a multiplication per score.
+#include "vqa_flash2.h"
+#include "vqa_paged_attn.h"
+
+namespace vqa {
+namespace paged {
+namespace chunk {
+
+using flash::Geom;
+using flash::u32x4_t;
+using flash2::Scores;
+
+constexpr int kBN = flash2::kBN;
+constexpr int kRows = flash2::kBM;
+constexpr int kWaves = 4;
+static_assert(kBN == kKeyStep, "a key tile is a key step");
+
+template <typename Tag, int D, bool kRaw>
+__global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan p) {
+    typedef Geom<D> G;
+    typedef flash2::Pipe<Tag, D, kWaves, kRaw> Pipe;
+    typedef typename Pipe::KDma KDma;
+    typedef typename Pipe::VDma VDma;
+    typedef typename Elem<Tag>::vec8 vec8;
+    static_assert(KDma::kRowsPerWave == 16, "a wave's rows of a tile lie in one page");
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = __builtin_amdgcn_readfirstlane((int)(blockIdx.x % (unsigned)a.Hkv));
+    const uint32_t lds0 = flash::lds_addr_of(smem);
+    auto s_k = [&](int par) { return lds0 + (uint32_t)((par & 1) * G::kTileBytes); };
+    auto s_v = [&](int par) { return lds0 + (uint32_t)((2 + (par & 1)) * G::kTileBytes); };
+
+    KDma kd;
+    VDma vd;
+    kd.init(wave, lane, a.kp.sn / 2);
+    vd.init(wave, lane, a.vp.sn / 2);
+    const char* k_head = a.kp.p + h * a.kp.sh;
+    const char* v_head = a.vp.p + h * a.vp.sh;
+
+    for_each_piece(a, p, (int)(blockIdx.x / (unsigned)a.Hkv), (int)(gridDim.x / (unsigned)a.Hkv), lane,
+                   [&](const Piece& u, int step, int n_steps, bool whole_tile, int slot_out) __attribute__((always_inline)) {
+        const Seq& q = u.q;
+        const int n_rows = q.n * a.G;  // of the sequence (fits 32 bits)
+        const int row0 = u.tile * kRows + wave * flash2::kWaveRows;
+        const int k_lo = step * kKeyStep;
+        const int k_end = (int)min((int64_t)(step + n_steps) * kKeyStep, (int64_t)q.keys);
+        const int n_iter = k_end > k_lo ? (k_end - k_lo + kBN - 1) / kBN : 0;
+
+        // ---- pages: `tab` holds 64 table entries from entry tab0 on, `valid` which of them are pages
+        const int32_t* table = a.g.table + (int64_t)u.s * a.g.table_ss;
+        const int in_page = (1 << a.g.page_shift) - 1;
+        int tab = 0, tab0 = -0x40000000;
+        uint64_t valid = 0;
+        struct Place {
+            const char *k, *v;  // this wave's first row of the tile
+            int last;           // its last row that is there, within 16 (at least 0)
+            bool there;         // every page of the tile is there
+        };
+        auto place = [&](int t) __attribute__((always_inline)) {  // (t increases from call to call)
+            const int j0 = k_lo + t * kBN;
+            const int c0 = j0 >> a.g.page_shift;
+            if (c0 - tab0 >= 64) {  // (a block of entries begins with a tile, and 64 is a multiple of a tile's pages)
+                tab0 = c0;
+                const int e = c0 + lane < a.g.width ? table[c0 + lane] : -1;
+                const bool ok = (unsigned)e < (unsigned)a.g.n_pages;
+                valid = __builtin_amdgcn_ballot_w64(ok);
+                tab = ok ? e : 0;  // (a page that is not there reads page 0; its keys are hidden)
+            }
+            Place x;
+            const int jw = j0 + 16 * wave;
+            const int j = jw < k_end ? jw : (k_end - 1) & ~15;  // rows behind the end repeat the last one
+            x.last = min(15, k_end - 1 - j);
+            const int64_t page = __builtin_amdgcn_readlane(tab, (j >> a.g.page_shift) - tab0);
+            const int64_t off = j & in_page;
+            x.k = k_head + page * a.kp.sp + off * a.kp.sn;
+            x.v = v_head + page * a.vp.sp + off * a.vp.sn;
+            const int c1 = (min(j0 + kBN, k_end) - 1) >> a.g.page_shift;
+            const uint64_t mask = (~0ull >> (63 - (c1 - c0))) << (c0 - tab0);
+            x.there = (valid & mask) == mask;
+            return x;
+        };
+        // which 16-row groups of tile t are there, bit by bit (rare)
+        auto groups_there = [&](int t) {
+            int bits = 0;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int j = k_lo + t * kBN + 16 * g;
+                if (j < k_end) bits |= page_of(a.g, u.s, j) >= 0 ? 1 << g : 0;
+            }
+            return bits;
+        };
+        // a tile copy as a block: rows behind the end repeat the last one
+        auto copy = [&](auto is_v, uint32_t tile, const char* rows, int last) __attribute__((always_inline)) {
+            constexpr bool kV = decltype(is_v)::value;
+            const int l = flash2::opaque_lane(lane);
+            const uint32_t sn = (uint32_t)(kV ? a.vp.sn : a.kp.sn);
+#pragma unroll
+            for (int i = 0; i < KDma::kInstr; ++i) {
+                const int r = i * G::kRowsPerInstr + l / G::kChunksPerRow;
+                const int chunk = (l % G::kChunksPerRow) ^ (kV ? G::swz_v(16 * wave + r) : G::swz_k(16 * wave + r));
+                flash::dma16_uniform(rows, (uint32_t)min(r, last) * sn + (uint32_t)chunk * 16u,
+                                     tile + (uint32_t)((16 * wave + i * G::kRowsPerInstr) * G::kRowBytes));
+            }
+        };
+        typedef std::false_type K;
+        typedef std::true_type V;
+
+        // ---- rows of this lane: what they see; the wave's common part
+        int tok[2];  // new token of each of the lane's two rows
+        flash2::Wave<Tag, D> w;
+        w.init();
+        w.c = a.scale_log2e;
+        Place now = {nullptr, nullptr, 0, true}, next = now;
+        if (n_iter > 0) {
+            now = place(0);
+            copy(K(), s_k(0), now.k, now.last);
+            copy(V(), s_v(0), now.v, now.last);
+            next = now;
+            if (n_iter > 1) {
+                next = place(1);
+                copy(K(), s_k(1), next.k, next.last);
+            }
+        }
+        const int t_first = min(row0, n_rows - 1) / a.G, t_last = min(row0 + flash2::kWaveRows - 1, n_rows - 1) / a.G;
+        const int all_hi = visible(a, q, t_first).hi, all_lo = visible(a, q, t_last).lo;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+            const int r = min(row0 + qb * 32 + (lane & 31), n_rows - 1);  // rows past the end are computed, never stored
+            const int t = r / a.G, g = r - t * a.G;
+            tok[qb] = t;
+            const uint16_t* src = a.q + (int64_t)(q.q0 + t) * a.q_st + (int64_t)(h * a.G + g) * a.q_sh + (lane >> 5) * 8;
+#pragma unroll
+            for (int kk = 0; kk < G::kKSteps; ++kk) w.q[qb].f[kk] = *reinterpret_cast<const vec8*>(src + kk * 16);
+            flash2::prescale_q<Tag, D>(w.q[qb], kRaw ? 1.f : a.scale_log2e);
+        }
+
+        Scores s_even, s_odd;
+        typename Pipe::Frags kf, vf;
+        float mx[2] = {-INFINITY, -INFINITY};
+        auto mask_tile = [&](Scores& sn, int t, bool there) __attribute__((always_inline)) {
+            const int n0 = k_lo + t * kBN;
+            if (there && n0 + kBN <= all_hi && n0 >= all_lo && t < n_iter) return;  // (wave-uniform)
+            flash2::mfma_settle(sn);
+            const int half = flash2::opaque_lane(lane) >> 5;
+            const int bits = t < n_iter ? (there ? 15 : groups_there(t)) : 0;
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) {
+                const Range x = visible(a, q, tok[qb]);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = n0 + kb * 32 + flash::key_of_reg(r, half);
+                        const bool seen = j < x.hi && j >= x.lo && ((bits >> (2 * kb + (r >> 3))) & 1);
+                        sn.s[qb][kb][r] = seen ? sn.s[qb][kb][r] : -INFINITY;
+                    }
+            }
+        };
+        const typename Pipe::TileRequest no_req{nullptr, 0};
+
+        if (n_iter > 0) {
+            flash::wait_tile_loads();
+            __syncthreads();
+            Pipe::k_head(kf, s_k(0), lane);
+            Pipe::template score_phase<true, false, false, false>(w, s_even, kf, s_odd, vf, 0u, lane, kd, no_req, vd, no_req);
+            mask_tile(s_even, 0, now.there);
+            Pipe::template pv_phase<false, true>(w, vf, s_odd, s_even, mx);
+        }
+        // Iteration t finishes tile t and scores tile t + 1; it requests K(t + 2) and V(t + 1).  `next` is the place of tile
+        // t + 1 when it begins.
+        auto iteration = [&](auto t_is_odd, auto ride, int t) __attribute__((always_inline)) {
+            constexpr int par = decltype(t_is_odd)::value ? 1 : 0;
+            constexpr bool kRide = decltype(ride)::value;
+            Scores& sc = par ? s_odd : s_even;
+            Scores& sn = par ? s_even : s_odd;
+            flash::wait_tile_loads();
+            __syncthreads();  // K(t + 1) and V(t) are complete; every wave is done with K(t) and V(t - 1)
+            Pipe::k_head(kf, s_k(par + 1), lane);
+            typename Pipe::TileRequest kr = no_req, vr = no_req;
+            const bool there = next.there;
+            if constexpr (kRide) {
+                vr.rows = next.v;
+                vr.lds = VDma::lds_of_wave(s_v(par + 1), wave);
+                next = place(t + 2);
+                kr.rows = next.k;
+                kr.lds = KDma::lds_of_wave(s_k(par), wave);
+            } else {
+                if (t + 1 < n_iter) copy(V(), s_v(par + 1), next.v, next.last);
+                if (t + 2 < n_iter) {
+                    next = place(t + 2);
+                    copy(K(), s_k(par), next.k, next.last);
+                }
+            }
+            Pipe::update_max(w, mx, sc);
+            Pipe::template score_phase<true, true, true, kRide>(w, sn, kf, sc, vf, s_v(par), lane, kd, kr, vd, vr);
+            mask_tile(sn, t + 1, there);
+            mx[0] = mx[1] = -INFINITY;
+            Pipe::template pv_phase<true, true>(w, vf, sc, sn, mx);
+        };
+        const int n_whole = (k_end - k_lo) / kBN;  // tiles with all 64 rows
+        int t = 0;
+        for (; t + 3 < n_whole; t += 2) {
+            iteration(std::false_type{}, std::true_type{}, t);
+            iteration(std::true_type{}, std::true_type{}, t + 1);
+        }
+        for (; t < n_iter; t += 2) {
+            iteration(std::false_type{}, std::false_type{}, t);
+            if (t + 1 < n_iter) iteration(std::true_type{}, std::false_type{}, t + 1);
+        }
+        Pipe::settle_o(w);
+        __syncthreads();  // no wave reads tiles any more
+
+        // ---- results.  A row that came out as infinity or NaN may have met one in a value it does not see (0 * inf): it is
+        // done again, key by key.
+        const int half = lane >> 5, n = lane & 31;
+        uint64_t bad = 0;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+            const float l = flash2::join_halves_sum(w.l[qb][0] + w.l[qb][1]);
+            const float m = kRaw && w.m[qb] != -INFINITY ? w.m[qb] * w.c : w.m[qb];
+            const int r = row0 + qb * 32 + n;
+            float probe = l;
+#pragma unroll
+            for (int db = 0; db < G::kDBlocks; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) probe += w.o[qb][db][i] * 0.f;
+            const uint64_t vote = __builtin_amdgcn_ballot_w64(!(probe < INFINITY) && r < n_rows);
+            bad |= ((vote | (vote >> 32)) & 0xffffffffull) << (32 * qb);
+            if (whole_tile) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                char* dst = smem + wave * Pipe::kStoreBytes + (qb * 32 + n) * Pipe::kStoreRowBytes;
+#pragma unroll
+                for (int db = 0; db < G::kDBlocks; ++db)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<uint2*>(dst + (db * 32 + 8 * g + 4 * half) * 2) =
+                            make_uint2(Elem<Tag>::pack2(w.o[qb][db][4 * g] * inv, w.o[qb][db][4 * g + 1] * inv),
+                                       Elem<Tag>::pack2(w.o[qb][db][4 * g + 2] * inv, w.o[qb][db][4 * g + 3] * inv));
+                if (a.lse != nullptr && half == 0 && r < n_rows) {
+                    const int t = r / a.G;
+                    a.lse[(int64_t)(q.q0 + t) * a.Hq + h * a.G + r - t * a.G] = l == 0.f ? -INFINITY : m + fast_log2(l);
+                }
+            } else if (r < n_rows) {
+                const int64_t at = ((int64_t)slot_out * a.Hkv + h) * kRows + wave * flash2::kWaveRows + qb * 32 + n;
+#pragma unroll
+                for (int db = 0; db < G::kDBlocks; ++db)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<float4*>(p.o + at * D + db * 32 + 8 * g + 4 * half) = make_float4(
+                            w.o[qb][db][4 * g], w.o[qb][db][4 * g + 1], w.o[qb][db][4 * g + 2], w.o[qb][db][4 * g + 3]);
+                if (half == 0) p.ml[at * 2] = m, p.ml[at * 2 + 1] = l;
+            }
+        }
+        if (whole_tile) {
+            wave_lds_sync();
+            constexpr int kLanesPerRow = G::kRowBytes / 16, kRowsPerInstr = 64 / kLanesPerRow;
+            const int c = lane % kLanesPerRow;
+#pragma unroll
+            for (int i = 0; i < flash2::kWaveRows / kRowsPerInstr; ++i) {
+                const int in = i * kRowsPerInstr + lane / kLanesPerRow, r = row0 + in;
+                const char* src = smem + wave * Pipe::kStoreBytes + in * Pipe::kStoreRowBytes + c * 16;
+                const uint2 x = *reinterpret_cast<const uint2*>(src), y = *reinterpret_cast<const uint2*>(src + 8);
+                if (r < n_rows) {
+                    const int t = r / a.G;
+                    *reinterpret_cast<uint4*>(a.out + (int64_t)(q.q0 + t) * a.o_st + (int64_t)(h * a.G + r - t * a.G) * a.o_sh +
+                                              c * 8) = make_uint4(x.x, x.y, y.x, y.y);
+                }
+            }
+        }
+        for (; bad; bad &= bad - 1) {
+            const int in = __builtin_ctzll(bad), r = row0 + in, t = r / a.G, hq = h * a.G + r - t * a.G;
+            const Range x = visible(a, q, t);
+            RowState<D> st;
+            row_by_lanes<Tag, D, false>(a, u.s, h, a.q + (int64_t)(q.q0 + t) * a.q_st + (int64_t)hq * a.q_sh,
+                                        max(k_lo, x.lo), min(k_end, x.hi), st, lane);
+            if (whole_tile) {
+                store_row<Tag, D>(a, st, q.q0 + t, hq, lane);
+            } else {
+                const int64_t at = ((int64_t)slot_out * a.Hkv + h) * kRows + wave * flash2::kWaveRows + in;
+#pragma unroll
+                for (int e = 0; e < D / 64; ++e) p.o[at * D + lane * (D / 64) + e] = st.o[e];
+                if (lane == 0) p.ml[at * 2] = st.m, p.ml[at * 2 + 1] = st.l;
+            }
+        }
+        __syncthreads();  // the staging area is free for the next piece's tiles
+    });
+}
+
+template <typename Tag, int D, bool kRaw>
+int launch(const AttnArgs& a, const Plan& p, int64_t grid, hipStream_t stream) {
+    constexpr int tiles = 4 * Geom<D>::kTileBytes;
+    constexpr int stage = kWaves * flash2::Pipe<Tag, D, kWaves, kRaw>::kStoreBytes;
+    constexpr int bytes = tiles > stage ? tiles : stage;
+    if (bytes > 64 * 1024)
+        if (int rc = raise_lds<chunk_kernel<Tag, D, kRaw>>(a.q, bytes)) return rc;
+    chunk_kernel<Tag, D, kRaw><<<dim3((unsigned)grid), kWaves * 64, bytes, stream>>>(a, p);
+    return launch_status();
+}
+
+}  // namespace chunk
+
+template <typename Tag>
+int launch_chunk(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream) {
+    if (e4m3) return VQA_ERR_BAD_ARGUMENT;
+    if (D == 128)
+        return a.lse ? chunk::launch<Tag, 128, true>(a, p, grid, stream) : chunk::launch<Tag, 128, false>(a, p, grid, stream);
+    return a.lse ? chunk::launch<Tag, 64, true>(a, p, grid, stream) : chunk::launch<Tag, 64, false>(a, p, grid, stream);
+}
+template int launch_chunk<bf16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);
+template int launch_chunk<f16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);
+
+}  // namespace paged
+}  // namespace vqa

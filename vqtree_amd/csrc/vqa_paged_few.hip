@@ -77,8 +77,9 @@ __device__ __forceinline__ float quads_sum(float x) {
     return x + __shfl_xor(x, 32, 64);
 }
 
-// Brings tiles of one wave.
-template <int D, bool kE4m3>
+// Brings tiles of one wave.  kOnce: no other tile reads these rows (all rows of a sequence fit one tile), so the loads are
+// marked non-temporal: 213 -> 189 us for 1.19 GB of 16-bit rows, 105 -> 95 us for 0.54 GB of e4m3 rows.
+template <int D, bool kE4m3, bool kOnce>
 struct Loader {
     typedef Geo<D, kE4m3> G;
     const char *k, *v;             // pools at the key head
@@ -175,10 +176,16 @@ struct Loader {
     template <int I>
     static __device__ __forceinline__ void issue(uint32_t dst, uint32_t off, const char* base) {
         // (a load may not follow the write of M0 directly)
-        asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
-                     :
-                     : "s"(dst), "n"(I * 1024), "v"(off), "s"(base)
-                     : "memory", "scc");
+        if constexpr (kOnce)
+            asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3 nt"
+                         :
+                         : "s"(dst), "n"(I * 1024), "v"(off), "s"(base)
+                         : "memory", "scc");
+        else
+            asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
+                         :
+                         : "s"(dst), "n"(I * 1024), "v"(off), "s"(base)
+                         : "memory", "scc");
     }
 };
 
@@ -203,31 +210,21 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
     const int n = lane & 15, quad = lane >> 4;
     const int h = __builtin_amdgcn_readfirstlane((int)(blockIdx.x % (unsigned)a.Hkv));
     const uint32_t lds0 = flash::lds_addr_of(smem);
-    const int me = (int)(blockIdx.x / (unsigned)a.Hkv), n_wgs = (int)(gridDim.x / (unsigned)a.Hkv);
-
-    Line line;
-    line.init(a, p, lane);
-    if (p.parts && me >= line.parts) return;
-    Loader<D, kE4m3> ld;
+    Loader<D, kE4m3, NB == 1> ld;
     ld.init(a, h, lds0 + (uint32_t)(wave * G::kWaveBytes), lane);
 
-    const int64_t begin = p.parts ? line.start(me) : me, end = p.parts ? line.start(me + 1) : line.total;
-    for (int64_t x = begin; x < end;) {
-        const Piece u = line.find(a, p, x, lane);
-        const Seq q = seq_of(a.g, u.s);
+    for_each_piece(a, p, (int)(blockIdx.x / (unsigned)a.Hkv), (int)(gridDim.x / (unsigned)a.Hkv), lane,
+                   [&](const Piece& u, int step, int n_steps, bool whole, int slot_out) __attribute__((always_inline)) {
+        const Seq& q = u.q;
         const int n_rows = min(kRows, q.n * a.G - u.tile * kRows);  // (a tile is of one sequence: fits 32 bits)
-        const int n_steps = p.parts ? (int)min((int64_t)(u.steps - u.from), end - x) : u.steps;
-        const bool whole = n_steps == u.steps;
-        const int slot_out = 2 * me + (x == begin ? 0 : 1);
-        x += p.parts ? n_steps : n_wgs;
-        const int u_lo = (u.first + u.from) * kKeyStep;
-        const int u_hi = __builtin_amdgcn_readfirstlane((int)min((int64_t)(u.first + u.from + n_steps) * kKeyStep, (int64_t)q.keys));
+        const int u_lo = step * kKeyStep;
+        const int u_hi = (int)min((int64_t)(step + n_steps) * kKeyStep, (int64_t)q.keys);
         // this wave's part, in tiles
         const int n_tiles = max(0, (u_hi - u_lo + kKeys - 1) / kKeys);
         const int t_lo = n_tiles * wave / kWaves, t_hi = n_tiles * (wave + 1) / kWaves;
 
         ld.sequence(a, u.s, u_hi);
-        typename Loader<D, kE4m3>::Place places[G::kRing];
+        typename Loader<D, kE4m3, NB == 1>::Place places[G::kRing];
         auto ask_k = [&](int t, int slot) __attribute__((always_inline)) {
             places[slot] = ld.place(a.g, u_lo + t * kKeys);
             ld.template request<false>(a, places[slot], slot);
@@ -497,8 +494,8 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
                 store_row<Tag, D>(a, st, q.q0 + t, hq, lane);
             }
         }
-        __syncthreads();  // the staging area is free for the next unit's tiles
-    }
+        __syncthreads();  // the staging area is free for the next piece's tiles
+    });
 }
 
 template <int D, bool kE4m3, int NB>

@@ -169,7 +169,7 @@ def attn_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, *, k_exp=None, v
     max_q = T if max_q_len is None else max(0, min(int(max_q_len), T))
     causal = 1 if causal else 0
     window = -1 if window is None else min(int(window), (1 << 31) - 1)
-    ws_bytes = _attn_workspace_bytes(T, S, Hq, Hkv, D, page, width, causal, window, max_q)
+    ws_bytes = _attn_workspace_bytes(T, S, Hq, Hkv, D, page, width, e4m3, causal, window, max_q)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     strides = _lib.strides_array(*q.stride()[:2], *strides, *exp_strides, table_stride, *out.stride()[:2])
     _launch("vqa_paged_attn_", dtype, dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exp), _ptr(v_exp),
