@@ -409,10 +409,16 @@ struct Pipe {
     typedef TileDma<D, false, NW> KDma;
     typedef TileDma<D, true, NW> VDma;
     static_assert(KDma::kInstr == VDma::kInstr && 2 * KDma::kInstr <= kScoreSlots, "tile copy does not fit the slots");
-    template <bool kMma, bool kExp, bool kVHead, bool kDma>
+    // rider(slot): anything else a caller wants to run in the shadow of the slot's MFMA.
+    struct NoRider {
+        template <typename I>
+        __device__ __forceinline__ void operator()(I) const {}
+    };
+    template <bool kMma, bool kExp, bool kVHead, bool kDma, typename Rider = NoRider>
     static __device__ __forceinline__ void score_phase(Wave<Tag, D>& w, Scores& sn, Frags& kf, const Scores& sc,
                                                        Frags& vf, uint32_t lds_v, int lane, const KDma& kd,
-                                                       const TileRequest& kr, const VDma& vd, const TileRequest& vr) {
+                                                       const TileRequest& kr, const VDma& vd, const TileRequest& vr,
+                                                       Rider&& rider = Rider{}) {
         constexpr int NI = KDma::kInstr;
         static_assert(kMma || !kDma, "the loads ride on the MFMA slots");
         static_for<kScoreSlots>([&](auto I) {
@@ -435,6 +441,7 @@ struct Pipe {
             }
             if constexpr (kDma && i < NI) kd.template fire<i>(kr.rows);
             if constexpr (kDma && i >= NI && i < 2 * NI) vd.template fire<i - NI>(vr.rows);
+            rider(I);
             if constexpr (kVHead && i == kScoreSlots - 3) v_head(vf, lds_v, lane);
             __builtin_amdgcn_sched_barrier(0);
         });

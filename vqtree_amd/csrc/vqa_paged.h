@@ -106,7 +106,8 @@ inline int make_pool(Pool* pool, const void* pages, const uint8_t* exps, const i
     *pool = Pool{(char*)pages, s[0] * size, s[1] * size, s[2] * size, e4m3 ? (uint8_t*)exps : nullptr, e4m3 ? es[0] : 0,
                  e4m3 ? es[1] : 0};
     // (the exponents of 16 rows are fetched as one piece)
-    if (e4m3 && (!aligned16(exps) || es[0] % 16 || es[1] % 16)) return VQA_ERR_MISALIGNED;
+    if (e4m3 && (!aligned16(exps) || es[0] % 16 || es[1] % 16 || es[0] < 0 || es[0] >= (int64_t(1) << 32)))
+        return VQA_ERR_MISALIGNED;
     if (!aligned16(pages) || pool->sp % 16 || pool->sh % 16 || pool->sn % 16) return VQA_ERR_MISALIGNED;
     // a row's offset inside its page is kept in 32 bits
     if (pool->sn < 0 || pool->sn * page >= (int64_t(1) << 31)) return VQA_ERR_MISALIGNED;

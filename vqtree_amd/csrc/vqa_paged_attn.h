@@ -145,27 +145,37 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& 
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Work.  The new rows of a sequence and the G query heads of a key head are one list of n * G rows (row r: new token
-// r / G, head r % G of the group), cut into tiles; a tile has as many key steps (64 keys) as its rows see.  With splits, the
-// steps of all tiles of a key head stand in one line and each of its `parts` workgroups takes an equal piece of it, wherever
-// tiles begin and end: the lengths are known on the device only, and however unequal they are (and whatever a recorded call
-// meets when it is replayed) all workgroups end together.  A piece that is not a whole tile leaves an unnormalised result,
-// which join_kernel puts together.  Without splits a workgroup takes whole tiles, the last (longest) ones of the sequences
-// first.  Every kernel of a call computes the same plan from the same numbers.
+// r / G, head r % G of the group), cut into tiles; a tile has as many key steps (64 keys) as its rows see.  The lengths are
+// known on the device only, so that is where the work of a key head is dealt out to its workgroups ("parts"), in one of three
+// ways, whichever ends first by the counts of steps and what a piece of a tile costs:
+//   kWhole  whole tiles, the last (longest) ones of the sequences first;
+//   kEven   every tile in equal pieces, one piece to a part: the shortest pieces that give no more of them than parts;
+//   kLine   the steps of all tiles stand in one line and every part takes an equal stretch of it, wherever tiles begin and
+//           end: perfect balance however unequal the lengths, at the price of two or more pieces in a part.
+// A piece that is not a whole tile leaves an unnormalised result, which join_kernel puts together.  Every workgroup computes
+// the same plan from the same numbers, and so does a recorded call that is replayed on new ones.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kKeyStep = 64;
 
 struct Plan {
-    int rows;       // rows of a tile
+    int rows;       // rows of a tile (a power of two)
     int lo, hi;     // sequences with lo <= n * G <= hi belong to this kernel
-    int parts;      // workgroups per key head that share the steps; 0: no splits
+    int parts;      // workgroups per key head; 0: no pieces, the grid has a workgroup for every tile there may be
     int min_steps;  // fewest steps worth a workgroup
+    int piece_cost, join_cost;  // of a piece of a tile, and of joining them, in steps
+    int even;       // kEven is worth looking for
+    int* joins;     // [parts][Hkv][kJoinInts]: the tile a part begins inside of, if it is the first part to do so
     float* o;       // partial results [2 * part + (not the part's first piece)][Hkv][rows][D], unnormalised
     float* ml;      // [..][rows][2]: maximum (base 2, scaled) and sum
 };
 
+// n_pieces (0: nothing to join) | first packed row of the sequence | first row of the tile | rows of the tile that exist |
+// part the tile begins in | 1 if it is not that part's first piece
+constexpr int kJoinInts = 8;
+
 __device__ __forceinline__ int tiles_of(const AttnArgs& a, const Plan& p, const Seq& q) {
     const int64_t rows = (int64_t)q.n * a.G;
-    return rows < 1 || rows < p.lo || rows > p.hi ? 0 : (int)((rows + p.rows - 1) / p.rows);
+    return rows < 1 || rows < p.lo || rows > p.hi ? 0 : (int)((rows + p.rows - 1) >> (31 - __builtin_clz(p.rows)));
 }
 // key steps [first, first + steps) of tile t; a tile that sees nothing has one (its result is still stored)
 __device__ __forceinline__ void steps_of(const AttnArgs& a, const Plan& p, const Seq& q, int t, int& first, int& steps) {
@@ -179,29 +189,56 @@ __device__ __forceinline__ int64_t lane64(int64_t x, int from) {  // (from: the 
     const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), from);
     return (int64_t)(((uint64_t)hi << 32) | lo);
 }
-__device__ __forceinline__ int scan32(int x, int lane) {  // sum over the lanes up to this one
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
-    return x;
+// A value of another lane of the same row of 16, or of the row(s) before, by data-parallel primitives (one instruction where a
+// shuffle through LDS takes a hundred clocks; these stand at the start of every call).  Lanes without a source get `none`.
+template <int kCtrl, int kRowMask = 0xf>
+__device__ __forceinline__ int dpp(int x, int none) {
+    return __builtin_amdgcn_update_dpp(none, x, kCtrl, kRowMask, 0xf, false);
 }
-__device__ __forceinline__ int64_t scan64(int64_t x, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t lo = __shfl_up((uint32_t)x, o, 64), hi = __shfl_up((uint32_t)(x >> 32), o, 64);
-        if (lane >= o) x += (int64_t)(((uint64_t)hi << 32) | lo);
-    }
-    return x;
+// running combination over the lanes: shifts by 1, 2, 4, 8 inside rows of 16, then the last lanes of rows 0 / 2 and of row 1
+template <typename F>
+__device__ __forceinline__ int scan_lanes(int x, int none, F f) {
+    x = f(x, dpp<0x111>(x, none));
+    x = f(x, dpp<0x112>(x, none));
+    x = f(x, dpp<0x114>(x, none));
+    x = f(x, dpp<0x118>(x, none));
+    x = f(x, dpp<0x142, 0xa>(x, none));
+    return f(x, dpp<0x143, 0xc>(x, none));
+}
+__device__ __forceinline__ int scan32(int x) {  // sum over the lanes up to this one
+    return scan_lanes(x, 0, [](int a, int b) { return a + b; });
+}
+template <int kCtrl, int kRowMask = 0xf>
+__device__ __forceinline__ int64_t dpp64(int64_t x) {
+    const uint32_t lo = (uint32_t)dpp<kCtrl, kRowMask>((int)(uint32_t)x, 0), hi = (uint32_t)dpp<kCtrl, kRowMask>((int)(x >> 32), 0);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t scan64(int64_t x) {
+    x += dpp64<0x111>(x);
+    x += dpp64<0x112>(x);
+    x += dpp64<0x114>(x);
+    x += dpp64<0x118>(x);
+    x += dpp64<0x142, 0xa>(x);
+    return x + dpp64<0x143, 0xc>(x);
+}
+__device__ __forceinline__ int wave_most(int x) {
+    return __builtin_amdgcn_readlane(scan_lanes(x, (int)0x80000000, [](int a, int b) { return max(a, b); }), 63);
+}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(scan32(x), 63); }
+// x * i / n, rounded down (x * i below 2^62)
+__device__ __forceinline__ int64_t mul_div(int64_t x, int i, int n) {
+    if (x < (1 << 22) && i <= 512) return (int64_t)((uint32_t)x * (uint32_t)i / (uint32_t)n);
+    return x * i / n;
 }
 
 struct Piece {
     int s, tile;       // sequence, row tile
     Seq q;
     int first, steps;  // key steps of the whole tile
-    int from;          // of them, where the position lies
+    int from;          // of them (kLine), or of its pieces (kEven), where the position lies
 };
+
+enum Deal : int { kWhole, kEven, kLine };
 
 // The line of one key head's tiles, held by a wave: 64 tiles at a time, one in each lane.
 struct Line {
@@ -209,10 +246,12 @@ struct Line {
     int s, t;             // of this lane's tile: sequence, tile of the sequence
     Seq q;
     int first, steps;     // its key steps (steps 0: there is no such tile)
-    int64_t before, sum;  // steps before this block of tiles; in it, up to and with this lane's
-    int64_t total;        // steps (with splits) or tiles of the whole line
+    int64_t before, sum;  // weights before this block of tiles; in it, up to and with this lane's
+    int64_t total;        // of the whole line
     int n_tiles;
     int parts;            // workgroups that share the line (at most p.parts)
+    int deal;             // weight of a tile: 1, its pieces, its steps
+    int per;              // kEven: longest piece
 
     // Tiles base .. base + 63: each lane looks for its tile in the running count of tiles over the sequences.
     __device__ __forceinline__ void block(const AttnArgs& a, const Plan& p, int base_, int lane) {
@@ -223,7 +262,7 @@ struct Line {
             Seq x = {0, 0, 0, 0};
             if (sb + lane < a.g.S) x = seq_of(a.g, sb + lane);
             const int mine = tiles_of(a, p, x);
-            const int upto = scan32(mine, lane);
+            const int upto = scan32(mine);
             const int here = __builtin_amdgcn_readlane(upto, 63);
             const int want = base + lane - seen;
             if (base + kWave > seen && base < seen + here) {  // (uniform: some lane's tile is one of these sequences')
@@ -240,28 +279,52 @@ struct Line {
             seen += here;
         }
         n_tiles = seen;
-        sum = scan64(p.parts ? steps : (steps > 0 ? 1 : 0), lane);
+        sum = scan64(deal == kLine ? steps : steps == 0 ? 0 : deal == kEven ? (steps + per - 1) / per : 1);
     }
     __device__ __forceinline__ void init(const AttnArgs& a, const Plan& p, int lane) {
+        deal = p.parts ? kLine : kWhole;
+        per = 1;
         block(a, p, 0, lane);
         before = 0;
         total = lane64(sum, 63);
         parts = 0;
-        if (!p.parts) {
-            total = n_tiles;
-            return;
-        }
-        if (n_tiles > kWave) {
-            for (int b = kWave; b < n_tiles; b += kWave) {
-                block(a, p, b, lane);
-                total += lane64(sum, 63);
+        if (p.parts) {
+            int longest = wave_most(steps);
+            if (n_tiles > kWave) {
+                for (int b = kWave; b < n_tiles; b += kWave) {
+                    block(a, p, b, lane);
+                    total += lane64(sum, 63);
+                    longest = max(longest, wave_most(steps));
+                }
+                block(a, p, 0, lane);
             }
-            block(a, p, 0, lane);
+            parts = total >= (int64_t)p.parts * p.min_steps ? p.parts : max(1, (int)total / p.min_steps);
+            // whole tiles, dealt out to all parts, take about as long as the longest one times the rounds
+            const int64_t whole = (int64_t)longest * ((n_tiles + p.parts - 1) / p.parts);
+            const int64_t fair = mul_div(total, 1, parts);
+            int64_t best = fair + (n_tiles > 1 ? 2 : 1) * p.piece_cost + p.join_cost;
+            if (whole <= best) deal = kWhole, best = whole;
+            if (p.even && n_tiles > 1 && n_tiles <= min(parts, kWave)) {
+                int lo = (int)fair, hi = longest;  // lo pieces: too many, hi: few enough
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) / 2;
+                    if (wave_total((steps + mid - 1) / mid) <= parts) hi = mid;
+                    else lo = mid;
+                }
+                if (hi < longest && hi + p.piece_cost + p.join_cost < best) deal = kEven, per = hi;
+            }
+            if (deal != kLine) {
+                block(a, p, 0, lane);
+                total = lane64(sum, 63);  // (kEven: one block of tiles)
+            }
         }
-        parts = (int)max((int64_t)1, min((int64_t)p.parts, total / p.min_steps));
+        if (deal == kWhole) total = n_tiles;
     }
-    __device__ __forceinline__ int64_t start(int i) const { return total * i / parts; }  // of part i
-    __device__ __forceinline__ int part_of(int64_t x) const { return (int)(((x + 1) * parts - 1) / total); }
+    __device__ __forceinline__ int64_t start(int i) const { return mul_div(total, i, parts); }  // kLine: of part i
+    __device__ __forceinline__ int part_of(int64_t x) const {
+        if (total < (1 << 22) && parts <= 512) return (int)((uint32_t)((x + 1) * parts - 1) / (uint32_t)total);
+        return (int)(((x + 1) * parts - 1) / total);
+    }
 
     // the tile at position x < total; positions of later calls do not decrease
     __device__ __forceinline__ Piece find(const AttnArgs& a, const Plan& p, int64_t x, int lane) {
@@ -277,41 +340,64 @@ struct Line {
                   __builtin_amdgcn_readlane(q.len, at), __builtin_amdgcn_readlane(q.keys, at)};
         r.first = __builtin_amdgcn_readlane(first, at);
         r.steps = __builtin_amdgcn_readlane(steps, at);
-        r.from = p.parts ? (int)(x - before - lane64(sum - steps, at)) : 0;
+        r.from = (int)(x - before - (at ? lane64(sum, at - 1) : 0));
         return r;
-    }
-    // position of tile number i < n_tiles, and its key steps
-    __device__ __forceinline__ int64_t start_of_tile(const AttnArgs& a, const Plan& p, int i, int& n_steps, int lane) {
-        while (i >= base + kWave) {
-            before += lane64(sum, 63);
-            block(a, p, base + kWave, lane);
-        }
-        n_steps = __builtin_amdgcn_readlane(steps, i - base);
-        return before + lane64(sum - steps, i - base);
     }
 };
 
 // What a workgroup does: calls work(piece, first step, steps, whole, place in the workspace) for each of its pieces.  (The
 // line's block is made again behind a piece, so that it takes no registers meanwhile.)
 template <typename F>
-__device__ __forceinline__ void for_each_piece(const AttnArgs& a, const Plan& p, int me, int n_wgs, int lane, F&& work) {
+__device__ __forceinline__ void for_each_piece(const AttnArgs& a, const Plan& p, int lane, F&& work) {
+    const int me = (int)(blockIdx.x / (unsigned)a.Hkv), n_wgs = (int)(gridDim.x / (unsigned)a.Hkv);
+    int* note = p.joins + blockIdx.x * kJoinInts;
+    if (p.parts && threadIdx.x == 0) note[0] = 0;
     Line line;
     line.init(a, p, lane);
-    if (p.parts && me >= line.parts) return;
-    const int64_t begin = p.parts ? line.start(me) : line.total - 1 - me;  // (whole tiles: the longest, last ones first)
-    const int64_t end = p.parts ? line.start(me + 1) : 0;
-    int64_t x = begin;
-    if (p.parts ? x >= end : x < 0) return;
+    const int deal = line.deal;
+    int64_t x = 0, end = 0;
+    if (deal == kLine) {
+        if (me < line.parts) x = line.start(me), end = line.start(me + 1);
+    } else if (deal == kEven) {
+        x = me, end = min(line.total, (int64_t)me + 1);
+    } else {
+        x = line.total - 1 - me;  // (downwards: the last ones first)
+    }
+    if (deal == kWhole ? x < 0 : x >= end) return;
+    const int64_t begin = x;
     for (;;) {
-        if (!p.parts && (x < line.base || x >= line.base + kWave)) {
+        if (deal == kWhole && (x < line.base || x >= line.base + kWave)) {
             line.before = x & ~(int64_t)(kWave - 1);
             line.block(a, p, (int)line.before, lane);
         }
         const Piece u = line.find(a, p, x, lane);
-        const int n = p.parts ? (int)min((int64_t)(u.steps - u.from), end - x) : u.steps;
-        work(u, u.first + u.from, n, n == u.steps, 2 * me + (x == begin ? 0 : 1));
-        x += p.parts ? n : -n_wgs;
-        if (p.parts ? x >= end : x < 0) return;
+        int from = 0, n = u.steps, pieces = 1, i0 = me, shift = 0;
+        if (deal == kLine) {
+            from = u.from;
+            n = (int)min((int64_t)(u.steps - from), end - x);
+            const int64_t tile = x - from;
+            i0 = line.part_of(tile);
+            pieces = line.part_of(tile + u.steps - 1) - i0 + 1;
+            shift = tile == line.start(i0) ? 0 : 1;
+        } else if (deal == kEven) {
+            pieces = (u.steps + line.per - 1) / line.per;
+            from = (int)mul_div(u.steps, u.from, pieces);
+            n = (int)mul_div(u.steps, u.from + 1, pieces) - from;
+            i0 = me - u.from;
+        }
+        if (pieces > 1 && x == begin && from > 0 && i0 == me - 1 && threadIdx.x == 0) {
+            note[0] = pieces;
+            note[1] = u.q.q0;
+            note[2] = u.tile * p.rows;
+            note[3] = min(p.rows, u.q.n * a.G - u.tile * p.rows);
+            note[4] = i0;
+            note[5] = shift;
+        }
+        work(u, u.first + from, n, pieces == 1, 2 * me + (x == begin ? 0 : 1));
+        if (deal == kLine) x += n;
+        else if (deal == kEven) x += 1;
+        else x -= n_wgs;
+        if (deal == kWhole ? x < 0 : x >= end) return;
         line.block(a, p, line.base, lane);
     }
 }

@@ -6,68 +6,106 @@
 namespace vqa {
 namespace paged {
 
-// Joins the splits of a row: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.  One workgroup per row and query head,
-// its waves share the splits (their partial rows are 512 bytes each, so what counts is how many are in flight).
-constexpr int kJoinWaves = 4;
+// Joins the pieces of a tile: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.  A tile in pieces holds the place where
+// some part begins, and the first such part has noted it; the rows of all noted tiles are dealt out to the waves.  What it
+// costs is latency -- partial results come from other XCDs' caches or from HBM, 1 - 2 us a round -- so a wave asks for kAhead
+// pieces of kRowsEach rows at once.
+constexpr int kJoinWaves = 8;
 
 template <typename Tag, int D>
 __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan few, Plan chunk) {
     constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = (int)(blockIdx.x / (unsigned)a.Hq), hq = (int)(blockIdx.x % (unsigned)a.Hq);
-    const int s = find_seq(a.g, row, lane);
-    if (s >= a.g.S) return;
-    const Seq q = seq_of(a.g, s);
-    if (row < q.q0 || row >= q.q0 + q.n) return;
-    const Plan p = tiles_of(a, few, q) ? few : chunk;
-    if (p.parts == 0) return;  // (whole tiles)
-    Line line;
-    line.init(a, p, lane);
-    int tile = 0;  // number of the row's tile: the tiles of the sequences before it, then its own
-    for (int base = 0; base < s; base += kWave) {
-        const int mine = base + lane < s ? tiles_of(a, p, seq_of(a.g, base + lane)) : 0;
-        tile += __builtin_amdgcn_readlane(scan32(mine, lane), 63);
+    constexpr int kAhead = 8, kRowsEach = 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Plan& p = few.parts == 0 || blockIdx.z ? chunk : few;
+    const int n_notes = p.parts * a.Hkv;
+    int64_t item = (int64_t)blockIdx.x * kJoinWaves + wave;  // number of the group of rows among all groups to join
+    int64_t before = 0;
+    for (int base = 0; base < n_notes; base += 64) {
+        int4 d = make_int4(0, 0, 0, 0);
+        int2 d2 = make_int2(0, 0);
+        if (base + lane < n_notes) {
+            const int* src = p.joins + (base + lane) * kJoinInts;
+            d = *reinterpret_cast<const int4*>(src);
+            d2 = *reinterpret_cast<const int2*>(src + 4);
+        }
+        const int mine = d.x ? (d.w + kRowsEach - 1) / kRowsEach : 0;
+        const int upto = scan32(mine);
+        const int64_t here = __builtin_amdgcn_readlane(upto, 63);
+        for (; item < before + here; item += (int64_t)gridDim.x * kJoinWaves) {
+            const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(item < before + upto));
+            // rows r0 .. of the tile
+            const int r0 = ((int)(item - before) - __builtin_amdgcn_readlane(upto - mine, at)) * kRowsEach;
+            const int n = __builtin_amdgcn_readlane(d.x, at), q0 = __builtin_amdgcn_readlane(d.y, at);
+            const int row0 = __builtin_amdgcn_readlane(d.z, at), n_rows = __builtin_amdgcn_readlane(d.w, at);
+            const int i0 = __builtin_amdgcn_readlane(d2.x, at), shift = __builtin_amdgcn_readlane(d2.y, at);
+            const int h = (base + at) % a.Hkv;
+            // piece k lies with part i0 + k; that of part i0 itself may be its second
+            const int64_t step = (int64_t)2 * a.Hkv * p.rows, skew = (int64_t)shift * a.Hkv * p.rows;
+            const int64_t first = (int64_t)i0 * step + (int64_t)h * p.rows;
+            auto place = [&](int k, int r) { return first + k * step + (k ? 0 : skew) + min(r0 + r, n_rows - 1); };
+            // lane 8 * r + k weighs piece k of row r (lanes from 32 on repeat those)
+            const int my_k = lane % kAhead, my_r = lane / kAhead % kRowsEach;
+            float m_run = -INFINITY, l_run = 0.f, o[kRowsEach][E];
+#pragma unroll
+            for (int r = 0; r < kRowsEach; ++r)
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[r][e] = 0.f;
+            for (int k0 = 0; k0 < n; k0 += kAhead) {
+                const int k = k0 + my_k;
+                const float2 ml = *reinterpret_cast<const float2*>(p.ml + place(min(k, n - 1), my_r) * 2);
+                float x[kAhead][kRowsEach][E];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+#pragma unroll
+                    for (int r = 0; r < kRowsEach; ++r)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) x[j][r][e] = 0.f;
+                    if (k0 + j < n) {  // (uniform)
+#pragma unroll
+                        for (int r = 0; r < kRowsEach; ++r)
+#pragma unroll
+                            for (int e = 0; e < E; ++e) x[j][r][e] = p.o[place(k0 + j, r) * D + lane * E + e];
+                    }
+                }
+                const float m = k < n ? ml.x : -INFINITY;
+                float top = m;
+#pragma unroll
+                for (int s = 1; s < kAhead; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+                top = fmaxf(top, m_run);
+                const float ref = top == -INFINITY ? 0.f : top;
+                const float alpha = fast_exp2(m_run - ref), f = fast_exp2(m - ref);
+                float l = k < n ? f * ml.y : 0.f;
+#pragma unroll
+                for (int s = 1; s < kAhead; s <<= 1) l += __shfl_xor(l, s, 64);
+                l_run = l_run * alpha + l;
+                m_run = top;
+#pragma unroll
+                for (int r = 0; r < kRowsEach; ++r) {
+                    const float al = __shfl(alpha, r * kAhead, 64);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[r][e] *= al;
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) {
+                        const float w = __shfl(f, r * kAhead + j, 64);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) o[r][e] += w * x[j][r][e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < kRowsEach; ++r) {
+                if (r0 + r >= n_rows) continue;
+                RowState<D> st;
+                st.m = __shfl(m_run, r * kAhead, 64), st.l = __shfl(l_run, r * kAhead, 64);
+#pragma unroll
+                for (int e = 0; e < E; ++e) st.o[e] = o[r][e];
+                const int rr = row0 + r0 + r, t = rr / a.G;
+                store_row<Tag, D>(a, st, q0 + t, h * a.G + rr - t * a.G, lane);
+            }
+        }
+        before += here;
     }
-    const int h = hq / a.G, r = (row - q.q0) * a.G + hq % a.G;
-    int n_steps;
-    const int64_t from = line.start_of_tile(a, p, tile + r / p.rows, n_steps, lane);
-    const int i0 = line.part_of(from), i1 = line.part_of(from + n_steps - 1);
-    if (i0 == i1) return;  // (one workgroup had the whole tile and has stored the result)
-    // the tile is the first piece of every part it reaches but perhaps the one it begins in
-    const int shift = from == line.start(i0) ? 0 : 1;
-    auto place = [&](int i) { return ((int64_t)(2 * i + (i == i0 ? shift : 0)) * a.Hkv + h) * p.rows + r % p.rows; };
-    float top = -INFINITY;
-    for (int i = i0 + lane; i <= i1; i += 64) top = fmaxf(top, p.ml[place(i) * 2]);
-    top = wave_max(top);
-    float o[E], l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-    for (int i = i0 + wave; i <= i1; i += kJoinWaves) {
-        const int64_t at = place(i);
-        const float m = p.ml[at * 2];
-        const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
-        l += f * p.ml[at * 2 + 1];
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += f * p.o[at * D + lane * E + e];
-    }
-    __shared__ float part[kJoinWaves][64][E + 1];
-#pragma unroll
-    for (int e = 0; e < E; ++e) part[wave][lane][e] = o[e];
-    part[wave][lane][E] = l;
-    __syncthreads();
-    if (wave != 0) return;
-    RowState<D> st;
-    st.m = top, st.l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) st.o[e] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWaves; ++w) {
-        st.l += part[w][lane][E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) st.o[e] += part[w][lane][e];
-    }
-    store_row<Tag, D>(a, st, row, hq, lane);
 }
 
 // How a call is cut up (host side; how many rows and keys there are is known on the device only).
@@ -83,6 +121,7 @@ constexpr int kFewRows = 64;        // sequences of more rows go to the chunk ke
 
 inline size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
 inline size_t o_bytes(const Plan& p, int Hkv, int D) { return round256((size_t)2 * p.parts * Hkv * p.rows * D * 4); }
+inline size_t join_bytes(const Plan& p, int Hkv) { return round256((size_t)p.parts * Hkv * kJoinInts * 4); }
 inline size_t ml_bytes(const Plan& p, int Hkv) { return round256((size_t)2 * p.parts * Hkv * p.rows * 8); }
 
 // keys: most keys a row can see, as far as the caller's numbers tell
@@ -91,21 +130,24 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
     Cut c{};
     const int64_t most = (int64_t)std::max(1, std::min(max_q, T)) * G;  // rows of a sequence
     const int64_t seqs = std::min(S, T), all = (int64_t)T * G;
-    const int limit = !e4m3 && most > kFewRows ? kFewRows : 0x7fffffff;
+    const int limit = most > kFewRows ? kFewRows : 0x7fffffff;
     const bool short_keys = keys <= (int64_t)kWholeSteps * kKeyStep;
-    auto plan = [&](int rows, int lo, int hi, int whole_from, int min_steps, Plan& p, int64_t& grid, size_t& bytes) {
+    auto plan = [&](int rows, int lo, int hi, int whole_from, Plan& p, int64_t& grid, size_t& bytes) {
         const int64_t rows_each = std::min<int64_t>(most, hi);
         const int64_t tiles = std::min(all / rows + seqs, seqs * ((rows_each + rows - 1) / rows));
         p.rows = rows, p.lo = lo, p.hi = hi;
         p.parts = tiles * Hkv >= whole_from || short_keys ? 0 : std::max(1, kCus / Hkv);
-        p.min_steps = min_steps;
         grid = (p.parts ? p.parts : tiles) * Hkv;
-        bytes = p.parts ? o_bytes(p, Hkv, D) + ml_bytes(p, Hkv) : 0;
+        bytes = o_bytes(p, Hkv, D) + ml_bytes(p, Hkv) + join_bytes(p, Hkv);
     };
     // (a hint that is too small keeps every sequence in the few-rows kernel; one that is too large costs an idle launch)
     if (!(most > limit && S == 1 && max_q >= T && all > kFewRows))
-        plan(std::min<int64_t>(most, limit) <= 16 ? 16 : 32, 1, limit, 8 * kCus, 8, c.few, c.few_grid, c.few_bytes);
-    if (most > limit) plan(256, limit + 1, 0x7fffffff, 4 * kCus, 4, c.chunk, c.chunk_grid, c.chunk_bytes);
+        // (next to chunks most of the others are single tokens)
+        plan(std::min<int64_t>(most, limit) <= 16 || (most > limit && G <= 16) ? 16 : 32, 1, limit, 8 * kCus, c.few, c.few_grid, c.few_bytes);
+    if (most > limit) plan(256, limit + 1, 0x7fffffff, 4 * kCus, c.chunk, c.chunk_grid, c.chunk_bytes);
+    // in key steps of about 1 us (few rows) and 2 us (chunks)
+    c.few.min_steps = 8, c.few.piece_cost = 2, c.few.join_cost = 2, c.few.even = 0;
+    c.chunk.min_steps = 4, c.chunk.piece_cost = 5, c.chunk.join_cost = 8, c.chunk.even = 1;
     return c;
 }
 
@@ -122,13 +164,15 @@ int run(const AttnArgs& a, Cut& c, void* ws, int D, bool e4m3, hipStream_t strea
         at += o_bytes(*p, a.Hkv, D);
         p->ml = (float*)at;
         at += ml_bytes(*p, a.Hkv);
+        p->joins = (int*)at;
+        at += join_bytes(*p, a.Hkv);
     }
     if (c.chunk.rows)
         if (int rc = launch_chunk<Tag>(a, c.chunk, D, e4m3, c.chunk_grid, stream)) return rc;
     if (c.few.rows)
         if (int rc = launch_few<Tag>(a, c.few, D, e4m3, c.few_grid, stream)) return rc;
     if (c.few.parts || c.chunk.parts) {
-        const dim3 grid((unsigned)((int64_t)a.g.T * a.Hq));
+        const dim3 grid(c.chunk.parts ? 2 * kCus : kCus, 1, c.few.parts && c.chunk.parts ? 2 : 1);
         if (D == 128)
             join_kernel<Tag, 128><<<grid, kJoinWaves * 64, 0, stream>>>(a, c.few, c.chunk);
         else

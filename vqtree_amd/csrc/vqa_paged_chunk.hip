@@ -6,6 +6,11 @@
 // Rows of a tile differ in what they see; masks are evaluated per element only on tiles where they do (diagonal, window
 // edge, end, missing pages).
 //
+// e4m3 rows go HBM -> LDS as they are, each wave its own 16 of a tile, and are widened to the element type on the way into the
+// tile buffers, once per workgroup: 8 conversions and two LDS writes per 1 KB and wave, dealt out over the score MFMAs (a
+// wave converting the fragments it needs itself would do that work four times).  Raw rows arrive one iteration ahead of
+// their conversion, which is one ahead of their use.
+//
 // kRaw (a call that asks for the log-sum-exp): scores are scaled in fp32 behind the product; otherwise the query is
 // pre-multiplied by scale * log2(e) and rounded once more, which saves a multiplication per score.
 #include "vqa_flash2.h"
@@ -24,7 +29,15 @@ constexpr int kRows = flash2::kBM;
 constexpr int kWaves = 4;
 static_assert(kBN == kKeyStep, "a key tile is a key step");
 
-template <typename Tag, int D, bool kRaw>
+// e4m3: raw rows of one wave and tile pair (K of one tile, V of the one before): 16 rows each, then their exponents
+template <int D>
+struct Raw {
+    static constexpr int kUnits = 16 * D / 1024;  // 1 KB each, per source
+    static constexpr int kExp = 2 * 16 * D;
+    static constexpr int kBytes = 2 * 16 * D + 64;
+};
+
+template <typename Tag, int D, bool kE4m3, bool kRaw>
 __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan p) {
     typedef Geom<D> G;
     typedef flash2::Pipe<Tag, D, kWaves, kRaw> Pipe;
@@ -42,12 +55,33 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
 
     KDma kd;
     VDma vd;
-    kd.init(wave, lane, a.kp.sn / 2);
-    vd.init(wave, lane, a.vp.sn / 2);
+    if constexpr (!kE4m3) {
+        kd.init(wave, lane, a.kp.sn / 2);
+        vd.init(wave, lane, a.vp.sn / 2);
+    }
     const char* k_head = a.kp.p + h * a.kp.sh;
     const char* v_head = a.vp.p + h * a.vp.sh;
+    typedef Raw<D> RawG;
+    auto s_raw = [&](int par) {
+        return lds0 + (uint32_t)(4 * G::kTileBytes + ((par & 1) * kWaves + wave) * RawG::kBytes);
+    };
 
-    for_each_piece(a, p, (int)(blockIdx.x / (unsigned)a.Hkv), (int)(gridDim.x / (unsigned)a.Hkv), lane,
+    // e4m3, per lane (piece l % kPieces of row l / kPieces of a unit): byte of a unit's pieces in the pools, where its first
+    // 16 widened bytes go in a tile, and the exponents' head (lane 0: keys, lane 1: values)
+    constexpr int kPieces = D / 16, kUnitRows = 1024 / D;
+    uint32_t k_raw = 0, v_raw = 0, k_dst = 0, v_dst = 0, e_step = 0;
+    const uint8_t* e_head = nullptr;
+    if constexpr (kE4m3) {
+        const int r = lane / kPieces, c = lane % kPieces, row = 16 * wave + r;
+        k_raw = (uint32_t)r * (uint32_t)a.kp.sn + (uint32_t)c * 16u;
+        v_raw = (uint32_t)r * (uint32_t)a.vp.sn + (uint32_t)c * 16u;
+        k_dst = (uint32_t)(row * G::kRowBytes + ((2 * c) ^ G::swz_k(row)) * 16);
+        v_dst = (uint32_t)(row * G::kRowBytes + ((2 * c) ^ G::swz_v(row)) * 16);
+        e_head = lane & 1 ? a.vp.e + h * a.vp.eh : a.kp.e + h * a.kp.eh;
+        e_step = (uint32_t)(lane & 1 ? a.vp.ep : a.kp.ep);  // (the host has checked that it fits)
+    }
+
+    for_each_piece(a, p, lane,
                    [&](const Piece& u, int step, int n_steps, bool whole_tile, int slot_out) __attribute__((always_inline)) {
         const Seq& q = u.q;
         const int n_rows = q.n * a.G;  // of the sequence (fits 32 bits)
@@ -56,39 +90,49 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
         const int k_end = (int)min((int64_t)(step + n_steps) * kKeyStep, (int64_t)q.keys);
         const int n_iter = k_end > k_lo ? (k_end - k_lo + kBN - 1) / kBN : 0;
 
-        // ---- pages: `tab` holds 64 table entries from entry tab0 on, `valid` which of them are pages
+        // ---- pages: lane i holds where page tab0 + i begins, at this key head; `missing` says which are not there
         const int32_t* table = a.g.table + (int64_t)u.s * a.g.table_ss;
         const int in_page = (1 << a.g.page_shift) - 1;
+        const uint32_t tile_pages = a.g.page_shift >= 6 ? 1u : a.g.page_shift == 5 ? 3u : 15u;  // a bit per page of a tile
+        int64_t k_at = 0, v_at = 0;
         int tab = 0, tab0 = -0x40000000;
-        uint64_t valid = 0;
+        uint64_t missing = 0;
         struct Place {
             const char *k, *v;  // this wave's first row of the tile
+            int page;           // the page it lies in, and its row there
+            uint32_t off;
             int last;           // its last row that is there, within 16 (at least 0)
             bool there;         // every page of the tile is there
         };
-        auto place = [&](int t) __attribute__((always_inline)) {  // (t increases from call to call)
+        // (t increases from call to call; kWhole: the tile has all 64 rows)
+        auto place = [&](auto whole, int t) __attribute__((always_inline)) {
+            constexpr bool kWhole = decltype(whole)::value;
             const int j0 = k_lo + t * kBN;
             const int c0 = j0 >> a.g.page_shift;
             if (c0 - tab0 >= 64) {  // (a block of entries begins with a tile, and 64 is a multiple of a tile's pages)
                 tab0 = c0;
                 const int e = c0 + lane < a.g.width ? table[c0 + lane] : -1;
                 const bool ok = (unsigned)e < (unsigned)a.g.n_pages;
-                valid = __builtin_amdgcn_ballot_w64(ok);
+                missing = ~__builtin_amdgcn_ballot_w64(ok);
                 tab = ok ? e : 0;  // (a page that is not there reads page 0; its keys are hidden)
+                k_at = (int64_t)(uintptr_t)k_head + (int64_t)tab * a.kp.sp;
+                v_at = (int64_t)(uintptr_t)v_head + (int64_t)tab * a.vp.sp;
             }
             Place x;
             const int jw = j0 + 16 * wave;
-            const int j = jw < k_end ? jw : (k_end - 1) & ~15;  // rows behind the end repeat the last one
-            x.last = min(15, k_end - 1 - j);
-            const int64_t page = __builtin_amdgcn_readlane(tab, (j >> a.g.page_shift) - tab0);
-            const int64_t off = j & in_page;
-            x.k = k_head + page * a.kp.sp + off * a.kp.sn;
-            x.v = v_head + page * a.vp.sp + off * a.vp.sn;
-            const int c1 = (min(j0 + kBN, k_end) - 1) >> a.g.page_shift;
-            const uint64_t mask = (~0ull >> (63 - (c1 - c0))) << (c0 - tab0);
-            x.there = (valid & mask) == mask;
+            const int j = kWhole || jw < k_end ? jw : (k_end - 1) & ~15;  // rows behind the end repeat the last one
+            x.last = kWhole ? 15 : min(15, k_end - 1 - j);
+            const int at = (j >> a.g.page_shift) - tab0;
+            x.off = (uint32_t)(j & in_page);  // (a row's offset inside its page fits 32 bits)
+            x.k = reinterpret_cast<const char*>((uintptr_t)lane64(k_at, at)) + x.off * (uint32_t)a.kp.sn;
+            x.v = reinterpret_cast<const char*>((uintptr_t)lane64(v_at, at)) + x.off * (uint32_t)a.vp.sn;
+            x.page = 0;
+            if constexpr (kE4m3) x.page = __builtin_amdgcn_readlane(tab, at);
+            x.there = ((uint32_t)(missing >> (c0 - tab0)) & tile_pages) == 0;
             return x;
         };
+        typedef std::true_type Whole;
+        typedef std::false_type Part;
         // which 16-row groups of tile t are there, bit by bit (rare)
         auto groups_there = [&](int t) {
             int bits = 0;
@@ -112,6 +156,62 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
                                      tile + (uint32_t)((16 * wave + i * G::kRowsPerInstr) * G::kRowBytes));
             }
         };
+        // ---- e4m3: raw rows in, widened rows out
+        auto ask_raw = [&](auto is_v, auto whole, auto unit, uint32_t raw, const Place& x) __attribute__((always_inline)) {
+            constexpr bool kV = decltype(is_v)::value;
+            constexpr int j = decltype(unit)::value;
+            const uint32_t sn = (uint32_t)(kV ? a.vp.sn : a.kp.sn);
+            const char* rows = kV ? x.v : x.k;
+            uint32_t off = kV ? v_raw : k_raw;
+            if constexpr (decltype(whole)::value) {
+                rows += j * kUnitRows * sn;
+            } else {
+                const int l = flash2::opaque_lane(lane);
+                off = (uint32_t)min(j * kUnitRows + l / kPieces, x.last) * sn + (uint32_t)(l % kPieces) * 16u;
+            }
+            asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
+                         :
+                         : "s"(raw), "n"((kV ? 16 * D : 0) + j * 1024), "v"(off), "s"(rows)
+                         : "memory", "scc");
+        };
+        // exponents of the 16 rows at kx (keys) and vx (values)
+        auto ask_exp = [&](uint32_t raw, const Place& kx, const Place& vx) __attribute__((always_inline)) {
+            const int l = flash2::opaque_lane(lane);
+            const uint8_t* src = e_head + (uint64_t)(uint32_t)(l & 1 ? vx.page : kx.page) * e_step + (l & 1 ? vx.off : kx.off);
+            if (l < 2) flash::dma16(src, raw + RawG::kExp);
+        };
+        struct Unit {
+            u32x4_t x;
+            uint32_t e;
+        };
+        typedef const __attribute__((address_space(3))) u32x4_t* lds16_in;
+        typedef __attribute__((address_space(3))) u32x4_t* lds16_out;
+        typedef const __attribute__((address_space(3))) uint8_t* lds8_in;
+        auto read_unit = [&](bool v, int j, uint32_t raw) __attribute__((always_inline)) {
+            const int l = flash2::opaque_lane(lane);
+            Unit r;
+            r.x = *(lds16_in)(uintptr_t)(raw + (uint32_t)((v ? 16 * D : 0) + j * 1024 + l * 16));
+            r.e = *(lds8_in)(uintptr_t)(raw + (uint32_t)(RawG::kExp + (v ? 16 : 0) + j * kUnitRows + l / kPieces));
+            return r;
+        };
+        // where the unit's first 16 bytes go (the second 16 lie at that address ^ 16): 8 rows on, the key tile's XOR has
+        // another bit, the value tile's has not
+        auto unit_dst = [&](bool v, int j, uint32_t tile) __attribute__((always_inline)) {
+            static_assert(RawG::kUnits <= 2, "the XOR of a third unit is not looked after");
+            return tile + (v ? v_dst : k_dst ^ (uint32_t)(j * 128)) + (uint32_t)(j * kUnitRows * G::kRowBytes);
+        };
+        auto widen_unit = [&](const Unit& r, uint32_t dst) __attribute__((always_inline)) {
+            const float f = factor_of((int)r.e);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint2 p0 = widen4<Tag>(r.x[2 * e], f), p1 = widen4<Tag>(r.x[2 * e + 1], f);
+                *(lds16_out)(uintptr_t)(dst ^ (uint32_t)(16 * e)) = u32x4_t{p0.x, p0.y, p1.x, p1.y};
+            }
+        };
+        auto widen_block = [&](bool v, uint32_t raw, uint32_t tile) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < RawG::kUnits; ++j) widen_unit(read_unit(v, j, raw), unit_dst(v, j, tile));
+        };
         typedef std::false_type K;
         typedef std::true_type V;
 
@@ -120,14 +220,42 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
         flash2::Wave<Tag, D> w;
         w.init();
         w.c = a.scale_log2e;
-        Place now = {nullptr, nullptr, 0, true}, next = now;
-        if (n_iter > 0) {
-            now = place(0);
+        Place now = {nullptr, nullptr, 0, 0, 0, true}, next = now, after = now;
+        if (kE4m3 && n_iter > 0) {
+            auto ask_all = [&](auto is_v, uint32_t raw, const Place& x) __attribute__((always_inline)) {
+                flash2::static_for<RawG::kUnits>([&](auto J) { ask_raw(is_v, Part(), J, raw, x); });
+            };
+            now = place(Part(), 0);
+            ask_all(K(), s_raw(0), now);
+            ask_all(V(), s_raw(0), now);
+            ask_exp(s_raw(0), now, now);
+            next = now;
+            if (n_iter > 1) {
+                next = place(Part(), 1);
+                ask_all(K(), s_raw(1), next);
+                ask_exp(s_raw(1), next, next);
+            }
+            flash::wait_tile_loads();
+            asm volatile("" ::: "memory");
+            widen_block(false, s_raw(0), s_k(0));
+            widen_block(true, s_raw(0), s_v(0));
+            widen_block(false, s_raw(1), s_k(1));
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            after = next;
+            if (n_iter > 1) ask_all(V(), s_raw(0), next);
+            if (n_iter > 2) {
+                after = place(Part(), 2);
+                ask_all(K(), s_raw(0), after);
+            }
+            ask_exp(s_raw(0), after, next);
+        }
+        if (!kE4m3 && n_iter > 0) {
+            now = place(Part(), 0);
             copy(K(), s_k(0), now.k, now.last);
             copy(V(), s_v(0), now.v, now.last);
             next = now;
             if (n_iter > 1) {
-                next = place(1);
+                next = place(Part(), 1);
                 copy(K(), s_k(1), next.k, next.last);
             }
         }
@@ -169,7 +297,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
         const typename Pipe::TileRequest no_req{nullptr, 0};
 
         if (n_iter > 0) {
-            flash::wait_tile_loads();
+            if constexpr (!kE4m3) flash::wait_tile_loads();
             __syncthreads();
             Pipe::k_head(kf, s_k(0), lane);
             Pipe::template score_phase<true, false, false, false>(w, s_even, kf, s_odd, vf, 0u, lane, kd, no_req, vd, no_req);
@@ -191,13 +319,13 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
             if constexpr (kRide) {
                 vr.rows = next.v;
                 vr.lds = VDma::lds_of_wave(s_v(par + 1), wave);
-                next = place(t + 2);
+                next = place(Whole(), t + 2);
                 kr.rows = next.k;
                 kr.lds = KDma::lds_of_wave(s_k(par), wave);
             } else {
                 if (t + 1 < n_iter) copy(V(), s_v(par + 1), next.v, next.last);
                 if (t + 2 < n_iter) {
-                    next = place(t + 2);
+                    next = place(Part(), t + 2);
                     copy(K(), s_k(par), next.k, next.last);
                 }
             }
@@ -207,15 +335,86 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
             mx[0] = mx[1] = -INFINITY;
             Pipe::template pv_phase<true, true>(w, vf, sc, sn, mx);
         };
-        const int n_whole = (k_end - k_lo) / kBN;  // tiles with all 64 rows
+        // e4m3: `next` and `after` are the places of tiles t + 1 and t + 2; the raw rows of K(t + 2) and V(t + 1) have arrived
+        // when iteration t begins and are widened in it, those of K(t + 3) and V(t + 2) are requested.
+        auto iteration8 = [&](auto t_is_odd, auto whole, int t) __attribute__((always_inline)) {
+            constexpr int par = decltype(t_is_odd)::value ? 1 : 0;
+            Scores& sc = par ? s_odd : s_even;
+            Scores& sn = par ? s_even : s_odd;
+            flash::wait_tile_loads();
+            __syncthreads();
+            Pipe::k_head(kf, s_k(par + 1), lane);
+            const bool there = next.there;
+            const Place v_of = after;  // tile t + 2
+            Place k_of = after;
+            constexpr bool kWhole = decltype(whole)::value;  // tiles t + 2 and t + 3 have all 64 rows
+            const bool more_v = kWhole || t + 2 < n_iter, more_k = kWhole || t + 3 < n_iter;
+            if (more_k) k_of = place(whole, t + 3);
+            const uint32_t raw_in = s_raw(par), raw_out = s_raw(par + 1);
+            Unit unit = read_unit(false, 0, raw_in), coming = unit;
+            uint32_t dst = 0;
+            float f = 0.f;
+            u32x4_t half;
+            Pipe::update_max(w, mx, sc);
+            constexpr int kU = 2 * RawG::kUnits;  // units in the order K .. V ..
+            static_assert(Pipe::kScoreSlots == 8 * kU, "a unit takes eight slots");
+            Pipe::template score_phase<true, true, true, false>(
+                w, sn, kf, sc, vf, s_v(par), lane, kd, no_req, vd, no_req, [&](auto I) __attribute__((always_inline)) {
+                    constexpr int i = decltype(I)::value, U = i / 8, s = i % 8;
+                    constexpr bool v = U >= RawG::kUnits;
+                    constexpr int j = U % RawG::kUnits;
+                    if constexpr (s == 0) {
+                        dst = unit_dst(v, j, v ? s_v(par + 1) : s_k(par));
+                        f = factor_of((int)unit.e);
+                        flash2::pin(f);
+                    }
+                    if constexpr (s == 1 || s == 2 || s == 4 || s == 5) {
+                        constexpr int word = s < 3 ? s - 1 : s - 2;
+                        const uint2 p = widen4<Tag>(unit.x[word], f);
+                        half[2 * (word & 1)] = p.x, half[2 * (word & 1) + 1] = p.y;
+                    }
+                    if constexpr (s == 3) *(lds16_out)(uintptr_t)dst = half;
+                    if constexpr (s == 6) *(lds16_out)(uintptr_t)(dst ^ 16u) = half;
+                    if constexpr (s == 4 && U + 1 < kU) {
+                        constexpr int n = U + 1;
+                        coming = read_unit(n >= RawG::kUnits, n % RawG::kUnits, raw_in);
+                    }
+                    if constexpr (s == 7) {
+                        unit = coming;
+                        if constexpr (v) {
+                            if (more_v) ask_raw(V(), whole, std::integral_constant<int, j>{}, raw_out, v_of);
+                        } else {
+                            if (more_k) ask_raw(K(), whole, std::integral_constant<int, j>{}, raw_out, k_of);
+                        }
+                        if constexpr (U == kU - 1)
+                            if (more_v) ask_exp(raw_out, k_of, v_of);
+                    }
+                });
+            mask_tile(sn, t + 1, there);
+            next = v_of, after = k_of;
+            mx[0] = mx[1] = -INFINITY;
+            Pipe::template pv_phase<true, true>(w, vf, sc, sn, mx);
+        };
         int t = 0;
-        for (; t + 3 < n_whole; t += 2) {
-            iteration(std::false_type{}, std::true_type{}, t);
-            iteration(std::true_type{}, std::true_type{}, t + 1);
-        }
-        for (; t < n_iter; t += 2) {
-            iteration(std::false_type{}, std::false_type{}, t);
-            if (t + 1 < n_iter) iteration(std::true_type{}, std::false_type{}, t + 1);
+        const int n_whole = (k_end - k_lo) / kBN;  // tiles with all 64 rows
+        if constexpr (kE4m3) {
+            for (; t + 4 < n_whole; t += 2) {
+                iteration8(std::false_type{}, Whole(), t);
+                iteration8(std::true_type{}, Whole(), t + 1);
+            }
+            for (; t < n_iter; t += 2) {
+                iteration8(std::false_type{}, Part(), t);
+                if (t + 1 < n_iter) iteration8(std::true_type{}, Part(), t + 1);
+            }
+        } else {
+            for (; t + 3 < n_whole; t += 2) {
+                iteration(std::false_type{}, std::true_type{}, t);
+                iteration(std::true_type{}, std::true_type{}, t + 1);
+            }
+            for (; t < n_iter; t += 2) {
+                iteration(std::false_type{}, std::false_type{}, t);
+                if (t + 1 < n_iter) iteration(std::true_type{}, std::false_type{}, t + 1);
+            }
         }
         Pipe::settle_o(w);
         __syncthreads();  // no wave reads tiles any more
@@ -281,7 +480,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
             const int in = __builtin_ctzll(bad), r = row0 + in, t = r / a.G, hq = h * a.G + r - t * a.G;
             const Range x = visible(a, q, t);
             RowState<D> st;
-            row_by_lanes<Tag, D, false>(a, u.s, h, a.q + (int64_t)(q.q0 + t) * a.q_st + (int64_t)hq * a.q_sh,
+            row_by_lanes<Tag, D, kE4m3>(a, u.s, h, a.q + (int64_t)(q.q0 + t) * a.q_st + (int64_t)hq * a.q_sh,
                                         max(k_lo, x.lo), min(k_end, x.hi), st, lane);
             if (whole_tile) {
                 store_row<Tag, D>(a, st, q.q0 + t, hq, lane);
@@ -296,25 +495,28 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
     });
 }
 
-template <typename Tag, int D, bool kRaw>
+template <typename Tag, int D, bool kE4m3, bool kRaw>
 int launch(const AttnArgs& a, const Plan& p, int64_t grid, hipStream_t stream) {
-    constexpr int tiles = 4 * Geom<D>::kTileBytes;
+    constexpr int tiles = 4 * Geom<D>::kTileBytes + (kE4m3 ? 2 * kWaves * Raw<D>::kBytes : 0);
     constexpr int stage = kWaves * flash2::Pipe<Tag, D, kWaves, kRaw>::kStoreBytes;
     constexpr int bytes = tiles > stage ? tiles : stage;
     if (bytes > 64 * 1024)
-        if (int rc = raise_lds<chunk_kernel<Tag, D, kRaw>>(a.q, bytes)) return rc;
-    chunk_kernel<Tag, D, kRaw><<<dim3((unsigned)grid), kWaves * 64, bytes, stream>>>(a, p);
+        if (int rc = raise_lds<chunk_kernel<Tag, D, kE4m3, kRaw>>(a.q, bytes)) return rc;
+    chunk_kernel<Tag, D, kE4m3, kRaw><<<dim3((unsigned)grid), kWaves * 64, bytes, stream>>>(a, p);
     return launch_status();
+}
+template <typename Tag, int D, bool kE4m3>
+int launch(const AttnArgs& a, const Plan& p, int64_t grid, hipStream_t stream) {
+    return a.lse ? launch<Tag, D, kE4m3, true>(a, p, grid, stream) : launch<Tag, D, kE4m3, false>(a, p, grid, stream);
 }
 
 }  // namespace chunk
 
 template <typename Tag>
 int launch_chunk(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream) {
-    if (e4m3) return VQA_ERR_BAD_ARGUMENT;
     if (D == 128)
-        return a.lse ? chunk::launch<Tag, 128, true>(a, p, grid, stream) : chunk::launch<Tag, 128, false>(a, p, grid, stream);
-    return a.lse ? chunk::launch<Tag, 64, true>(a, p, grid, stream) : chunk::launch<Tag, 64, false>(a, p, grid, stream);
+        return e4m3 ? chunk::launch<Tag, 128, true>(a, p, grid, stream) : chunk::launch<Tag, 128, false>(a, p, grid, stream);
+    return e4m3 ? chunk::launch<Tag, 64, true>(a, p, grid, stream) : chunk::launch<Tag, 64, false>(a, p, grid, stream);
 }
 template int launch_chunk<bf16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);
 template int launch_chunk<f16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);

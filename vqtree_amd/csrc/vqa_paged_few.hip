@@ -213,7 +213,7 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
     Loader<D, kE4m3, NB == 1> ld;
     ld.init(a, h, lds0 + (uint32_t)(wave * G::kWaveBytes), lane);
 
-    for_each_piece(a, p, (int)(blockIdx.x / (unsigned)a.Hkv), (int)(gridDim.x / (unsigned)a.Hkv), lane,
+    for_each_piece(a, p, lane,
                    [&](const Piece& u, int step, int n_steps, bool whole, int slot_out) __attribute__((always_inline)) {
         const Seq& q = u.q;
         const int n_rows = min(kRows, q.n * a.G - u.tile * kRows);  // (a tile is of one sequence: fits 32 bits)
