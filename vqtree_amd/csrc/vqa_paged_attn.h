@@ -6,6 +6,7 @@
 // lse = -inf.
 #pragma once
 
+#include <atomic>
 #include <mutex>
 
 #include "vqa_paged.h"
@@ -406,16 +407,18 @@ __device__ __forceinline__ void for_each_piece(const AttnArgs& a, const Plan& p,
 template <auto kKernel>
 int raise_lds(const void* operand, int bytes) {
     static std::mutex mutex;
-    static bool raised[kMaxDevices] = {};
+    static std::atomic<bool> raised[kMaxDevices];
     int dev = 0;
+    if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < kMaxDevices && raised[dev].load(std::memory_order_acquire))
+        return VQA_OK;
     if (int rc = device_of_pointer(operand, &dev)) return rc;
     std::lock_guard<std::mutex> lock(mutex);
-    if (!raised[dev]) {
-        if (hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
-            hipSuccess)
-            return VQA_ERR_LAUNCH_FAILED;
-        raised[dev] = true;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+        hipSuccess) {
+        (void)hipGetLastError();
+        return VQA_ERR_LAUNCH_FAILED;
     }
+    raised[dev].store(true, std::memory_order_release);
     return VQA_OK;
 }
 
