@@ -21,14 +21,22 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan 
     const int n_notes = p.parts * a.Hkv;
     int64_t item = (int64_t)blockIdx.x * kJoinWaves + wave;  // number of the group of rows among all groups to join
     int64_t before = 0;
-    for (int base = 0; base < n_notes; base += 64) {
-        int4 d = make_int4(0, 0, 0, 0);
-        int2 d2 = make_int2(0, 0);
-        if (base + lane < n_notes) {
-            const int* src = p.joins + (base + lane) * kJoinInts;
-            d = *reinterpret_cast<const int4*>(src);
-            d2 = *reinterpret_cast<const int2*>(src + 4);
-        }
+    for (int base4 = 0; base4 < n_notes; base4 += 256) {
+    // (the notes of up to 256 parts are asked for at once: there are no more where a part is a compute unit)
+    int4 notes[4];
+    int2 more[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const int* src = p.joins + (int64_t)min(base4 + b * 64 + lane, n_notes - 1) * kJoinInts;
+        notes[b] = *reinterpret_cast<const int4*>(src);
+        more[b] = *reinterpret_cast<const int2*>(src + 4);
+        if (base4 + b * 64 + lane >= n_notes) notes[b].x = 0;
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const int base = base4 + b * 64;
+        const int4 d = notes[b];
+        const int2 d2 = more[b];
         const int mine = d.x ? (d.w + kRowsEach - 1) / kRowsEach : 0;
         const int upto = scan32(mine);
         const int64_t here = __builtin_amdgcn_readlane(upto, 63);
@@ -106,6 +114,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(AttnArgs a, Plan 
         }
         before += here;
     }
+    }
 }
 
 // How a call is cut up (host side; how many rows and keys there are is known on the device only).
@@ -147,7 +156,7 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
     if (most > limit) plan(256, limit + 1, 0x7fffffff, 4 * kCus, c.chunk, c.chunk_grid, c.chunk_bytes);
     // in key steps of about 1 us (few rows) and 2 us (chunks)
     c.few.min_steps = 8, c.few.piece_cost = 2, c.few.join_cost = 2, c.few.even = 0;
-    c.chunk.min_steps = 4, c.chunk.piece_cost = 5, c.chunk.join_cost = 8, c.chunk.even = 1;
+    c.chunk.min_steps = 4, c.chunk.piece_cost = 8, c.chunk.join_cost = 10, c.chunk.even = 1;
     return c;
 }
 

@@ -220,6 +220,18 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
         flash2::Wave<Tag, D> w;
         w.init();
         w.c = a.scale_log2e;
+        // (the queries are asked for before the table and the first tiles, which depend on it)
+        const int t_first = min(row0, n_rows - 1) / a.G, t_last = min(row0 + flash2::kWaveRows - 1, n_rows - 1) / a.G;
+        const int all_hi = visible(a, q, t_first).hi, all_lo = visible(a, q, t_last).lo;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+            const int r = min(row0 + qb * 32 + (lane & 31), n_rows - 1);  // rows past the end are computed, never stored
+            const int t = r / a.G, g = r - t * a.G;
+            tok[qb] = t;
+            const uint16_t* src = a.q + (int64_t)(q.q0 + t) * a.q_st + (int64_t)(h * a.G + g) * a.q_sh + (lane >> 5) * 8;
+#pragma unroll
+            for (int kk = 0; kk < G::kKSteps; ++kk) w.q[qb].f[kk] = *reinterpret_cast<const vec8*>(src + kk * 16);
+        }
         Place now = {nullptr, nullptr, 0, 0, 0, true}, next = now, after = now;
         if (kE4m3 && n_iter > 0) {
             auto ask_all = [&](auto is_v, uint32_t raw, const Place& x) __attribute__((always_inline)) {
@@ -259,18 +271,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
                 copy(K(), s_k(1), next.k, next.last);
             }
         }
-        const int t_first = min(row0, n_rows - 1) / a.G, t_last = min(row0 + flash2::kWaveRows - 1, n_rows - 1) / a.G;
-        const int all_hi = visible(a, q, t_first).hi, all_lo = visible(a, q, t_last).lo;
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-            const int r = min(row0 + qb * 32 + (lane & 31), n_rows - 1);  // rows past the end are computed, never stored
-            const int t = r / a.G, g = r - t * a.G;
-            tok[qb] = t;
-            const uint16_t* src = a.q + (int64_t)(q.q0 + t) * a.q_st + (int64_t)(h * a.G + g) * a.q_sh + (lane >> 5) * 8;
-#pragma unroll
-            for (int kk = 0; kk < G::kKSteps; ++kk) w.q[qb].f[kk] = *reinterpret_cast<const vec8*>(src + kk * 16);
-            flash2::prescale_q<Tag, D>(w.q[qb], kRaw ? 1.f : a.scale_log2e);
-        }
+        flash2::prescale_q<Tag, D>(w.q[0], kRaw ? 1.f : a.scale_log2e);
+        flash2::prescale_q<Tag, D>(w.q[1], kRaw ? 1.f : a.scale_log2e);
 
         Scores s_even, s_odd;
         typename Pipe::Frags kf, vf;
@@ -464,14 +466,17 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
             wave_lds_sync();
             constexpr int kLanesPerRow = G::kRowBytes / 16, kRowsPerInstr = 64 / kLanesPerRow;
             const int c = lane % kLanesPerRow;
+            const int t0 = row0 / a.G, g0 = row0 - t0 * a.G;
+            const float inv_g = 1.f / (float)a.G;
 #pragma unroll
             for (int i = 0; i < flash2::kWaveRows / kRowsPerInstr; ++i) {
                 const int in = i * kRowsPerInstr + lane / kLanesPerRow, r = row0 + in;
                 const char* src = smem + wave * Pipe::kStoreBytes + in * Pipe::kStoreRowBytes + c * 16;
                 const uint2 x = *reinterpret_cast<const uint2*>(src), y = *reinterpret_cast<const uint2*>(src + 8);
                 if (r < n_rows) {
-                    const int t = r / a.G;
-                    *reinterpret_cast<uint4*>(a.out + (int64_t)(q.q0 + t) * a.o_st + (int64_t)(h * a.G + r - t * a.G) * a.o_sh +
+                    // (small numbers: exact in fp32, and half a step away from the next whole one)
+                    const int z = g0 + in, dt = (int)(((float)z + 0.5f) * inv_g);
+                    *reinterpret_cast<uint4*>(a.out + (int64_t)(q.q0 + t0 + dt) * a.o_st + (int64_t)(h * a.G + z - dt * a.G) * a.o_sh +
                                               c * 8) = make_uint4(x.x, x.y, y.x, y.y);
                 }
             }
