@@ -6,8 +6,6 @@ softmax * |v| and Z = the largest sum of |q_d k_d| * scale of a row:
   * scores are fp32 sums of D exact products, in the order of the matrix pipe: (D + 2) * u * Z each, which moves a
     weight by twice that (numerator and denominator), so 2 (D + 2) u Z * A; the long sums over N keys: 2 (N + 64) u * A, and exp2
     itself a few u: 16 u * A;
-  * where the query is multiplied by the scale and rounded to the element type before the products (long chunks without
-    lse): another eps * Z on a score, 2 eps Z * A;
   * fp16 has a smallest step of 2^-24: half of it per probability and result, N * 2^-25 * max|v| + 2^-25.
 The log-sum-exp is fp32 throughout: ((D + 2) Z + 2 (N + 64) + 16) * log2(e) * u, plus 2 u |lse|.
 """
@@ -74,17 +72,16 @@ class Cache:
               max_q_len, flush=True)
         got = self.attend(causal=causal, window=window, return_lse=lse, softmax_scale=softmax_scale, max_q_len=max_q_len)
         torch.cuda.synchronize()
-        compare(got if lse else (got, None), self.want(causal=causal, window=window, softmax_scale=softmax_scale), self,
-                prescaled=not lse)
+        compare(got if lse else (got, None), self.want(causal=causal, window=window, softmax_scale=softmax_scale), self)
 
 
-def compare(got, want, c, prescaled=False, rows=slice(None)):
+def compare(got, want, c, rows=slice(None)):
     out, lse = got
     w_out, w_lse, A, Z = (x[rows] for x in want)
     eps = torch.finfo(c.dtype).eps / 2
     N, D = max(c.lens + [1]), c.D
     Z = Z[..., None]
-    tol = (2 * eps + (2 * (D + 2) * Z + 2 * (N + 64) + 16) * U + (2 * eps * Z if prescaled else 0)) * A
+    tol = (2 * eps + (2 * (D + 2) * Z + 2 * (N + 64) + 16) * U) * A
     if c.dtype == torch.float16:
         tol = tol + N * 2.0**-25 * float(c.v.float().abs().nan_to_num(0, 0, 0).max()) + 2.0**-25
     err = (out.double().cpu()[rows] - w_out).abs()

@@ -15,8 +15,10 @@
 //
 // e4m3: keys are widened to the element type by v_cvt_scalef32_pk_* with their row's factor (a lane reads one key); values
 // are widened without factor, always to bf16 (exact), and the factor of the key goes to the probability instead, since a lane
-// then holds 8 keys of one d.  With f16 queries the scaled probability is split into two bf16 numbers (16 bits together), so
-// that neither f16's range nor bf16's 8 bits limit it.
+// then holds 8 keys of one d.
+//
+// Where the P.V product is in bf16, a probability is split into two bf16 numbers (16 bits together): the matrix pipe has the
+// time, and the output's error against 64 bits falls from 1.4 times that of its own rounding to 1.0 times.
 #include "vqa_flash2.h"
 #include "vqa_paged_attn.h"
 
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
     typedef typename Elem<Tag>::vec8 vec8;
     typedef typename std::conditional<kE4m3, bf16_tag, Tag>::type PTag;  // element type of the P.V product
     typedef typename Elem<PTag>::vec8 pvec8;
-    constexpr bool kSplitP = kE4m3 && std::is_same<Tag, f16_tag>::value;
+    constexpr bool kSplitP = std::is_same<PTag, bf16_tag>::value;
     constexpr int kRows = 16 * NB;
     constexpr int kStageRow = D + 4;  // floats; the padding spreads a column of rows over the banks
     typedef const __attribute__((address_space(3))) u32x4_t* lds16_ptr;
