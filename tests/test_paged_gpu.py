@@ -124,6 +124,77 @@ def test_attention(lengths, form):
     c.check(causal=False)
 
 
+DEALS = {  # new, past, Hkv, G, D, page: how the work is dealt out (few-rows kernel / chunk kernel)
+    "one_tile_many_parts": ([90], [3000], 2, 1, 128, 16),
+    "tiles_in_equal_pieces": ([600], [4200], 2, 1, 64, 64),
+    "line_of_tiles": ([70] * 5, [4300, 4200, 4100, 4000, 3900], 32, 1, 64, 128),
+    "line_of_single_tokens": ([1] * 9, [5000, 10, 2500, 0, 7000, 300, 4000, 1999, 63], 4, 2, 64, 16),
+    "more_than_64_sequences": ([1, 0, 2] * 50, list(range(0, 1500, 10)), 2, 4, 64, 32),
+    "more_than_64_tiles": ([33, 70, 1] * 24, [i % 90 for i in range(72)], 1, 2, 64, 16),
+    "long_tiles_beyond_64": ([70] * 66, [2100 + i for i in range(66)], 1, 1, 64, 256),
+    "no_keys_at_all": ([100, 1], [0, 0], 2, 2, 64, 16),
+    "large_pages": ([65, 1], [5000, 4097], 2, 1, 64, 4096),
+}
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("deal", DEALS, ids=str)
+def test_ways_of_dealing_out(deal, e4m3):
+    new, past, Hkv, G, D, page = DEALS[deal]
+    c = Cache(new, past, Hkv=Hkv, G=G, D=D, page=page, e4m3=e4m3, seed=20, spread=2.0)
+    if deal == "no_keys_at_all":
+        c.kv_lens.zero_()
+        c.lens = [0, 0]
+        out, lse = c.attend(return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+        return
+    want = c.want()
+    for max_q in (None, max(new), 1):  # (the last hint is wrong where there are chunks: slower, not wrong)
+        got = c.attend(return_lse=True, max_q_len=max_q)
+        torch.cuda.synchronize()
+        print(deal, e4m3, max_q, flush=True)
+        compare(got, want, c)
+
+
+@pytest.mark.parametrize("new", [[1], [80]])
+def test_offsets_beyond_32_bits(new):
+    """Pages that lie more than 4 GiB into the pools (and exponents far in): read, written and attended."""
+    H, D, page, n_pages = 8, 128, 64, 36000
+    c = Cache(new, [300], Hkv=H, D=D, page=page, seed=21)
+    k, v = (torch.empty(n_pages, H, page, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    assert k.numel() * 2 > 2**32
+    high = c.table.clone()
+    for i in range(high.shape[1]):
+        p = int(c.table[0, i])
+        if p >= 0:
+            high[0, i] = n_pages - 1 - p
+            k[n_pages - 1 - p], v[n_pages - 1 - p] = c.k[p].to(DEV), c.v[p].to(DEV)
+    out, lse = P.attn_paged(c.q.to(DEV), k, v, high.to(DEV), c.cu.to(DEV), c.kv_lens.to(DEV), return_lse=True)
+    compare((out, lse), c.want(), c)
+    rk, rv = P.paged_read(k, v, high.to(DEV), c.kv_lens.to(DEV), c.lens[0])
+    assert torch.equal(rk[0].double().cpu(), O.rows_of(c.k, None, c.table[0], c.lens[0])[0])
+    x = torch.randn(sum(new), H, D).to(torch.bfloat16)
+    P.paged_write(x.to(DEV), x.to(DEV), k, v, high.to(DEV), c.cu.to(DEV), c.kv_lens.to(DEV))
+    rk, rv = P.paged_read(k, v, high.to(DEV), c.kv_lens.to(DEV), c.lens[0])
+    assert torch.equal(rv[0, :, 300:].cpu(), x.transpose(0, 1)) and torch.equal(rk[0, :, 300:].cpu(), x.transpose(0, 1))
+
+
+@pytest.mark.parametrize("window", [0, 1, 63, 64, 129])
+def test_windows(window):
+    for e4m3 in (False, True):
+        c = Cache([70, 3], [200, 500], D=64, page=16, G=2, e4m3=e4m3, seed=22)
+        c.check(window=window)
+
+
+@pytest.mark.parametrize("scale", [1e-6, 1.0, 30.0])
+def test_scales(scale):
+    """Flat, sharp and one-hot softmax: the tolerance is that of the scores the scale gives."""
+    for new in ([1], [100]):
+        c = Cache(new, [700], D=64, page=16, seed=23)
+        got = c.attend(softmax_scale=scale, return_lse=True)
+        compare(got, c.want(softmax_scale=scale), c)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # writing and reading
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -341,10 +412,12 @@ def test_another_stream_and_two_calls_at_once():
     compare(gots[1], b.want(), b)
 
 
+@pytest.mark.parametrize("width", [64, 400])
 @pytest.mark.parametrize("new", [[1, 1, 1], [130, 1, 20]])
-def test_recorded_step_replays_on_new_lengths(new):
-    """A whole step -- write, then attend -- recorded once: lengths, tables and rows change between the replays."""
-    H, G, D, page, S, width = 2, 2, 128, 16, 3, 64
+def test_recorded_step_replays_on_new_lengths(new, width):
+    """A whole step -- write, then attend -- recorded once: lengths, tables and rows change between the replays (and with
+    the wide table the way the work is dealt out)."""
+    H, G, D, page, S = 2, 2, 128, 16, 3
     T = sum(new)
     g = torch.Generator().manual_seed(12)
     pools = [torch.zeros(S * width, H, page, D, dtype=torch.float8_e4m3fn, device=DEV) for _ in range(2)]
@@ -367,7 +440,8 @@ def test_recorded_step_replays_on_new_lengths(new):
     for i in range(4):
         for x in (q, k, v):
             x.copy_(torch.randn(x.shape, generator=g))
-        lens.copy_(torch.tensor([n * (i + 1) + 100 * s * (i % 2) for s, n in enumerate(new)], dtype=torch.int32))
+        far = 100 if width == 64 else 2900
+        lens.copy_(torch.tensor([n * (i + 1) + far * s * (i % 2) for s, n in enumerate(new)], dtype=torch.int32))
         graph.replay()
         got = out.clone(), lse.clone()
         again = step()  # (writes the same rows to the same places)

@@ -200,7 +200,7 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
     if (Hkv < 1 || Hq < 1 || Hq % Hkv || Hq > 65535 || (int64_t)T * Hq > (int64_t(1) << 31) - 1) return VQA_ERR_BAD_SHAPE;
     if (D != 64 && D != 128) return VQA_ERR_UNSUPPORTED_HEAD_DIM;
     if (window >= 0 && !causal) return VQA_ERR_BAD_ARGUMENT;
-    if (!(scale > 0.f) || !(scale <= 3e38f)) return VQA_ERR_BAD_ARGUMENT;
+    if (!(scale > 0.f) || !(scale < 2e38f)) return VQA_ERR_BAD_ARGUMENT;  // (times log2(e) it has to stay finite)
     AttnArgs a{};
     if (int rc = make_seqs(&a.g, cu, lens, table, st[12], S, T, width, n_pages, page)) return rc;
     if (int rc = make_pool(&a.kp, k_pages, k_exp, st + 2, st + 8, e4m3, page)) return rc;

@@ -188,11 +188,12 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
         typedef const __attribute__((address_space(3))) u32x4_t* lds16_in;
         typedef __attribute__((address_space(3))) u32x4_t* lds16_out;
         typedef const __attribute__((address_space(3))) uint8_t* lds8_in;
-        auto read_unit = [&](bool v, int j, uint32_t raw) __attribute__((always_inline)) {
+        // (rows behind the last one repeat it, so its exponent goes with them: what stands behind it may be anything)
+        auto read_unit = [&](bool v, int j, uint32_t raw, int last) __attribute__((always_inline)) {
             const int l = flash2::opaque_lane(lane);
             Unit r;
             r.x = *(lds16_in)(uintptr_t)(raw + (uint32_t)((v ? 16 * D : 0) + j * 1024 + l * 16));
-            r.e = *(lds8_in)(uintptr_t)(raw + (uint32_t)(RawG::kExp + (v ? 16 : 0) + j * kUnitRows + l / kPieces));
+            r.e = *(lds8_in)(uintptr_t)(raw + (uint32_t)(RawG::kExp + (v ? 16 : 0) + min(j * kUnitRows + l / kPieces, last)));
             return r;
         };
         // where the unit's first 16 bytes go (the second 16 lie at that address ^ 16): 8 rows on, the key tile's XOR has
@@ -209,9 +210,9 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
                 *(lds16_out)(uintptr_t)(dst ^ (uint32_t)(16 * e)) = u32x4_t{p0.x, p0.y, p1.x, p1.y};
             }
         };
-        auto widen_block = [&](bool v, uint32_t raw, uint32_t tile) __attribute__((always_inline)) {
+        auto widen_block = [&](bool v, uint32_t raw, uint32_t tile, int last) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < RawG::kUnits; ++j) widen_unit(read_unit(v, j, raw), unit_dst(v, j, tile));
+            for (int j = 0; j < RawG::kUnits; ++j) widen_unit(read_unit(v, j, raw, last), unit_dst(v, j, tile));
         };
         typedef std::false_type K;
         typedef std::true_type V;
@@ -250,9 +251,9 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
             }
             flash::wait_tile_loads();
             asm volatile("" ::: "memory");
-            widen_block(false, s_raw(0), s_k(0));
-            widen_block(true, s_raw(0), s_v(0));
-            widen_block(false, s_raw(1), s_k(1));
+            widen_block(false, s_raw(0), s_k(0), now.last);
+            widen_block(true, s_raw(0), s_v(0), now.last);
+            widen_block(false, s_raw(1), s_k(1), next.last);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             after = next;
             if (n_iter > 1) ask_all(V(), s_raw(0), next);
@@ -360,7 +361,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
             const bool more_v = kWhole || t + 2 < n_iter, more_k = kWhole || t + 3 < n_iter;
             if (more_k) k_of = place(whole, t + 3);
             const uint32_t raw_in = s_raw(par), raw_out = s_raw(par + 1);
-            Unit unit = read_unit(false, 0, raw_in), coming = unit;
+            const int k_last = kWhole ? 15 : after.last, v_last = kWhole ? 15 : next.last;  // of K(t + 2) and V(t + 1)
+            Unit unit = read_unit(false, 0, raw_in, k_last), coming = unit;
             uint32_t dst = 0;
             float f = 0.f;
             u32x4_t half;
@@ -386,7 +388,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
                     if constexpr (s == 6) *(lds16_out)(uintptr_t)(dst ^ 16u) = half;
                     if constexpr (s == 4 && U + 1 < kU) {
                         constexpr int n = U + 1;
-                        coming = read_unit(n >= RawG::kUnits, n % RawG::kUnits, raw_in);
+                        coming = read_unit(n >= RawG::kUnits, n % RawG::kUnits, raw_in, n >= RawG::kUnits ? v_last : k_last);
                     }
                     if constexpr (s == 7) {
                         unit = coming;
