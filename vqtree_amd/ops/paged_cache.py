@@ -16,7 +16,6 @@ brings one token per sequence, chunks of prompts, or both.  `paged_read` gives t
 the other operators take.  Lengths and tables are read on the device when the kernels run: a step recorded into a HIP
 graph replays on new ones.  Sequences of one call must not write to the same page (they may read the same one).
 """
-import functools
 import math
 
 import torch
@@ -27,8 +26,20 @@ from ._common import SUFFIX, last_dim_contiguous
 E4M3 = torch.float8_e4m3fn
 
 
-# A generation step is a few microseconds of GPU work, so the host side counts: attributes are read once, the device is
-# switched only where it has to be.
+# A generation step is a few microseconds of GPU work, so the host side counts.  What follows from shapes, strides, types and
+# options alone -- the checks, the strides array, the workspace's size -- is worked out once for each combination of them and
+# kept (_PLANS); a call then looks that up, checks the devices, and hands over the addresses.
+_PLANS = {}
+_MOST_PLANS = 4096
+
+
+def _remember(key, plan):
+    if len(_PLANS) >= _MOST_PLANS:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
+
+
 def _check_pools(k_pages, v_pages, k_exp, v_exp, dtype):
     """(e4m3, page shape, strides of the pools, strides of the exponents)"""
     shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
@@ -64,24 +75,26 @@ def _check_seqs(block_table, kv_lens, cu_q=None):
     return S, width, stride[0]
 
 
-def _check_devices(*tensors):
-    """index of the device all of them are on"""
-    dev = tensors[0].get_device()
+def _check_devices(dev, *tensors):
+    """every tensor is on GPU `dev` (an index; -1: the CPU)"""
     for t in tensors:
         if t is not None and t.get_device() != dev:
-            _lib.require_gpu(t, tensors[0])
+            _lib.require_gpu(t, *tensors)
             raise AssertionError("All tensors must be on the same device")
-    _lib.require_gpu(tensors[0])
-    return dev
+    if dev < 0:
+        _lib.require_gpu(*tensors)
 
 
 def _ptr(x):
     return None if x is None else x.data_ptr()
 
 
-def _launch(name, dtype, dev, *args):
-    """Calls the entry point of the element type on the current stream of device `dev`."""
-    fn = getattr(_lib.load(), name + SUFFIX[dtype])
+def _sig(x):
+    return None if x is None else (x.shape, x.stride(), x.dtype)
+
+
+def _launch(fn, dev, *args):
+    """Calls an entry point on the current stream of device `dev`."""
     if torch.cuda.current_device() == dev:
         rc = fn(*args, _lib.raw_stream(dev))
     else:
@@ -91,9 +104,8 @@ def _launch(name, dtype, dev, *args):
         _lib.check(rc)
 
 
-@functools.lru_cache(maxsize=1024)
-def _attn_workspace_bytes(*sizes):
-    return _lib.load().vqa_paged_attn_workspace_bytes(*sizes)
+def _entry(name, dtype):
+    return getattr(_lib.load(), name + SUFFIX[dtype])
 
 
 def paged_write(k, v, k_pages, v_pages, block_table, cu_q, kv_lens, *, k_exp=None, v_exp=None):
@@ -102,39 +114,62 @@ def paged_write(k, v, k_pages, v_pages, block_table, cu_q, kv_lens, *, k_exp=Non
     power of two that brings it into e4m3's +-448 and rounded to the nearest; NaN stays NaN, infinities and magnitudes
     beyond 1.875 * 2^15 (fp16) or 1.875 * 2^127 (bf16) are stored as that.  Rows behind the last sequence, before
     position 0, behind the table's last page or on a page that is not there are skipped."""
+    key = ("w", k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, k_pages.shape, k_pages.stride(), k_pages.dtype,
+           v_pages.shape, v_pages.stride(), v_pages.dtype, block_table.shape, block_table.stride(), block_table.dtype,
+           cu_q.shape, cu_q.stride(), cu_q.dtype, kv_lens.shape, kv_lens.stride(), kv_lens.dtype, _sig(k_exp), _sig(v_exp))
+    plan = _PLANS.get(key) or _remember(key, _plan_write(k, v, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp))
+    dev = k.get_device()
+    _check_devices(dev, k, v, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp)
+    fn, tail = plan
+    if tail is None:  # a last dimension with gaps, or nothing to do
+        if k.numel() and cu_q.numel() > 1:
+            paged_write(*last_dim_contiguous(k, v), k_pages, v_pages, block_table, cu_q, kv_lens, k_exp=k_exp, v_exp=v_exp)
+        return
+    _launch(fn, dev, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exp), _ptr(v_exp),
+            block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), *tail)
+
+
+def _plan_write(k, v, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp):
     shape, dtype = k.shape, k.dtype
     assert len(shape) == 3 and shape == v.shape and dtype == v.dtype, "k and v must be [T,H,D] of one type"
     T, H, D = shape
     e4m3, pages, strides, exp_strides = _check_pools(k_pages, v_pages, k_exp, v_exp, dtype)
     assert pages[1] == H and pages[3] == D, "k, v and the pages must have the same heads"
     S, width, table_stride = _check_seqs(block_table, kv_lens, cu_q)
-    dev = _check_devices(k, v, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp)
-    if T == 0 or S == 0:
-        return
-    k, v = last_dim_contiguous(k, v)
+    if T == 0 or S == 0 or k.stride(2) != 1 or v.stride(2) != 1:
+        return None, None
     strides = _lib.strides_array(*k.stride()[:2], *v.stride()[:2], *strides, *exp_strides, table_stride)
-    _launch("vqa_paged_write_", dtype, dev, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exp),
-            _ptr(v_exp), block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, S, H, D, pages[2], pages[0], width,
-            e4m3, strides)
+    return _entry("vqa_paged_write_", dtype), (T, S, H, D, pages[2], pages[0], width, e4m3, strides)
 
 
 def paged_read(k_pages, v_pages, block_table, kv_lens, n, *, k_exp=None, v_exp=None, dtype=None):
     """(k, v) [S,Hkv,n,D]: the first n rows of every sequence as plain tensors, zeros from kv_lens[s] on and on pages that
     are not there.  `dtype`: the element type of the result (8-bit pages: required; else the pages' own)."""
+    key = ("r", k_pages.shape, k_pages.stride(), k_pages.dtype, v_pages.shape, v_pages.stride(), v_pages.dtype,
+           block_table.shape, block_table.stride(), block_table.dtype, kv_lens.shape, kv_lens.stride(), kv_lens.dtype,
+           _sig(k_exp), _sig(v_exp), n, dtype)
+    plan = _PLANS.get(key) or _remember(key, _plan_read(k_pages, v_pages, block_table, kv_lens, n, k_exp, v_exp, dtype))
+    dev = k_pages.get_device()
+    _check_devices(dev, k_pages, v_pages, block_table, kv_lens, k_exp, v_exp)
+    fn, shape, dtype, tail = plan
+    k, v = k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+    if tail is not None:
+        _launch(fn, dev, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exp), _ptr(v_exp), block_table.data_ptr(),
+                kv_lens.data_ptr(), k.data_ptr(), v.data_ptr(), *tail)
+    return k, v
+
+
+def _plan_read(k_pages, v_pages, block_table, kv_lens, n, k_exp, v_exp, dtype):
     dtype = k_pages.dtype if dtype is None else dtype
     e4m3, pages, strides, exp_strides = _check_pools(k_pages, v_pages, k_exp, v_exp, dtype)
     S, width, table_stride = _check_seqs(block_table, kv_lens)
     assert n >= 0, "the number of rows must not be negative"
-    dev = _check_devices(k_pages, v_pages, block_table, kv_lens, k_exp, v_exp)
     P, H, page, D = pages
-    k = torch.empty((S, H, n, D), dtype=dtype, device=k_pages.device)
-    v = torch.empty_like(k)
-    if k.numel() == 0:
-        return k, v
-    strides = _lib.strides_array(*strides, *exp_strides, table_stride, *k.stride()[:3], *v.stride()[:3])
-    _launch("vqa_paged_read_", dtype, dev, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exp), _ptr(v_exp),
-            block_table.data_ptr(), kv_lens.data_ptr(), k.data_ptr(), v.data_ptr(), S, H, n, D, page, P, width, e4m3, strides)
-    return k, v
+    if S == 0 or n == 0 or H == 0:
+        return None, (S, H, n, D), dtype, None
+    out = (H * n * D, n * D, D)
+    strides = _lib.strides_array(*strides, *exp_strides, table_stride, *out, *out)
+    return _entry("vqa_paged_read_", dtype), (S, H, n, D), dtype, (S, H, n, D, page, P, width, e4m3, strides)
 
 
 def attn_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, *, k_exp=None, v_exp=None, softmax_scale=None,
@@ -147,6 +182,31 @@ def attn_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, *, k_exp=None, v
     return_lse, the base-2 log-sum-exp [T,Hq] fp32: a state `merge_state_in_place` can combine.  A row that sees no key
     gets 0 and -inf; rows behind the last sequence are left as they are (`out`: the buffer to write to).
     `max_q_len`: the most new tokens any sequence has, where the caller knows it; it steers the choice of kernels only."""
+    key = ("a", q.shape, q.stride(), q.dtype, k_pages.shape, k_pages.stride(), k_pages.dtype, v_pages.shape,
+           v_pages.stride(), v_pages.dtype, block_table.shape, block_table.stride(), block_table.dtype, cu_q.shape,
+           cu_q.stride(), cu_q.dtype, kv_lens.shape, kv_lens.stride(), kv_lens.dtype, _sig(k_exp), _sig(v_exp), _sig(out),
+           softmax_scale, causal, window, max_q_len)
+    plan = _PLANS.get(key) or _remember(key, _plan_attn(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp,
+                                                        softmax_scale, causal, window, max_q_len, out))
+    dev = q.get_device()
+    _check_devices(dev, q, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp, out)
+    fn, ws_bytes, tail = plan
+    if tail is None and q.numel() and kv_lens.numel():  # a last dimension with gaps
+        return attn_paged(q.contiguous(), k_pages, v_pages, block_table, cu_q, kv_lens, k_exp=k_exp, v_exp=v_exp,
+                          softmax_scale=softmax_scale, causal=causal, window=window, return_lse=return_lse,
+                          max_q_len=max_q_len, out=out)
+    if out is None:
+        out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
+    if tail is not None:
+        ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+        _launch(fn, dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exp), _ptr(v_exp),
+                block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(ws), ws_bytes,
+                *tail)
+    return (out, lse) if return_lse else out
+
+
+def _plan_attn(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp, softmax_scale, causal, window, max_q_len, out):
     shape, dtype = q.shape, q.dtype
     assert len(shape) == 3, "q must be [T,H,D]"
     T, Hq, D = shape
@@ -159,20 +219,14 @@ def attn_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, *, k_exp=None, v
     softmax_scale = softmax_scale or 1.0 / math.sqrt(D)
     assert softmax_scale > 0, "the softmax scale must be positive"
     assert out is None or (out.shape == shape and out.dtype == dtype and out.stride(2) == 1)
-    dev = _check_devices(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp, out)
-    (q,) = last_dim_contiguous(q)
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    if T == 0 or S == 0:
-        return (out, lse) if return_lse else out
+    if T == 0 or S == 0 or q.stride(2) != 1:
+        return None, 0, None
+    lib = _lib.load()
     max_q = T if max_q_len is None else max(0, min(int(max_q_len), T))
     causal = 1 if causal else 0
     window = -1 if window is None else min(int(window), (1 << 31) - 1)
-    ws_bytes = _attn_workspace_bytes(T, S, Hq, Hkv, D, page, width, e4m3, causal, window, max_q)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    strides = _lib.strides_array(*q.stride()[:2], *strides, *exp_strides, table_stride, *out.stride()[:2])
-    _launch("vqa_paged_attn_", dtype, dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_exp), _ptr(v_exp),
-            block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(ws), ws_bytes, T, S,
-            Hq, Hkv, D, page, P, width, e4m3, strides, causal, window, max_q, softmax_scale)
-    return (out, lse) if return_lse else out
+    ws_bytes = lib.vqa_paged_attn_workspace_bytes(T, S, Hq, Hkv, D, page, width, e4m3, causal, window, max_q)
+    out_strides = (Hq * D, D) if out is None else out.stride()[:2]
+    strides = _lib.strides_array(*q.stride()[:2], *strides, *exp_strides, table_stride, *out_strides)
+    return _entry("vqa_paged_attn_", dtype), ws_bytes, (T, S, Hq, Hkv, D, page, P, width, e4m3, strides, causal, window,
+                                                        max_q, softmax_scale)
