@@ -1,9 +1,12 @@
 // Writing new rows into the paged cache (vqa_paged_write_*) and reading it back as plain tensors (vqa_paged_read_*).
 //
-// Both move bytes.  Writing, a lane holds 16 elements of a row (8 lanes a row at head dim 128): with 8, which makes every load
-// one contiguous kilobyte, the quantiser's instructions per byte cost more than the loads gain (53 against 43 us for 8192
-// rows of 32 heads).  Reading, a lane holds 8, so that a wave stores contiguous kilobytes, past the caches: 105 us for 756 MB
-// (149 us with ordinary stores, 214 us with 16 elements per lane).
+// Both move bytes; MI355X copies large tensors at 4.84 TB/s (read and written) and reads them at about 7 TB/s.
+//   Writing, a lane holds 16 elements of a row (8 lanes a row at head dim 128): with 8, which makes every load one contiguous
+// kilobyte, the quantiser's instructions per byte cost more than the loads gain (53 against 43 us for 8192 rows of 32 heads, keys
+// and values, in a loop over one input).  Workgroups go over the heads first (43 -> 40 us), stores past the caches (47 -> 44 us
+// in a loop over several inputs: 4.6 TB/s).
+//   Reading, a lane holds 8 elements, so that a wave stores contiguous kilobytes, and past the caches: 756 MB in 134 us,
+// 5.6 TB/s (in a loop over one input 105 us; 149 with ordinary stores, 214 with 16 elements per lane).
 //
 // 8-bit rows.  The factor of a row is the smallest power of two 2^e with max |x| <= 448 * 2^e, 448 being the largest e4m3
 // number, so nothing saturates; the quotient is exact in fp32 and is rounded once, to the nearest e4m3 number (ties to even).
@@ -35,9 +38,9 @@ __device__ __forceinline__ void store_piece(const Pool& pool, const Seqs& g, con
                                             int piece, bool live, int lanes_per_row) {
     if (pool.e == nullptr) {  // (uniform)
         if (live) {
-            uint4* dst = reinterpret_cast<uint4*>(row_of(pool, g, page, h, j) + piece * 32);
-            dst[0] = x.a;
-            dst[1] = x.b;
+            char* dst = row_of(pool, g, page, h, j) + piece * 32;
+            store_stream16(dst, x.a);
+            store_stream16(dst + 16, x.b);
         }
         return;
     }
@@ -63,7 +66,7 @@ __device__ __forceinline__ void store_piece(const Pool& pool, const Seqs& g, con
         out[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inv, f[4 * i + 3] * inv, r, true);
     }
     if (live) {
-        *reinterpret_cast<uint4*>(row_of(pool, g, page, h, j) + piece * 16) = make_uint4(out[0], out[1], out[2], out[3]);
+        store_stream16(row_of(pool, g, page, h, j) + piece * 16, make_uint4(out[0], out[1], out[2], out[3]));
         if (piece == 0) *exp_of(pool, g, page, h, j) = (uint8_t)(e + 127);
     }
 }
