@@ -376,6 +376,11 @@ def test_numbers_out_of_range_do_no_harm():
     c.cu = torch.tensor([0, -5, 2**31 - 1, -(2**31)], dtype=torch.int32)
     c.attend()
     torch.cuda.synchronize()
+    # overlapping claims: a row goes to the first sequence that names it
+    c.cu = torch.tensor([0, 44, 4, 48], dtype=torch.int32)
+    got = c.attend(return_lse=True)
+    c.cu = torch.tensor([0, 44, 44, 48], dtype=torch.int32)
+    compare(got, c.want(), c)
 
 
 # ---------------------------------------------------------------------------------------------------------------------

@@ -254,14 +254,19 @@ struct Line {
     int deal;             // weight of a tile: 1, its pieces, its steps
     int per;              // kEven: longest piece
 
-    // Tiles base .. base + 63: each lane looks for its tile in the running count of tiles over the sequences.
+    // Tiles base .. base + 63: each lane looks for its tile in the running count of tiles over the sequences.  A sequence's
+    // rows begin where all before it have ended, whatever cu says: no row belongs to two, so there are no more tiles than rows.
     __device__ __forceinline__ void block(const AttnArgs& a, const Plan& p, int base_, int lane) {
         base = base_;
         steps = 0, first = 0, s = 0, t = 0, q = Seq{0, 0, 0, 0};
-        int seen = 0;
+        int seen = 0, ended = 0;
         for (int sb = 0; sb < a.g.S; sb += kWave) {
             Seq x = {0, 0, 0, 0};
             if (sb + lane < a.g.S) x = seq_of(a.g, sb + lane);
+            const int from = max(scan_lanes(x.q0, 0, [](int a, int b) { return max(a, b); }), ended);
+            x.n = max(x.q0 + x.n - from, 0);
+            x.q0 = from;
+            ended = __builtin_amdgcn_readlane(from, 63);
             const int mine = tiles_of(a, p, x);
             const int upto = scan32(mine);
             const int here = __builtin_amdgcn_readlane(upto, 63);
@@ -280,6 +285,9 @@ struct Line {
             seen += here;
         }
         n_tiles = seen;
+        weigh();
+    }
+    __device__ __forceinline__ void weigh() {
         sum = scan64(deal == kLine ? steps : steps == 0 ? 0 : deal == kEven ? (steps + per - 1) / per : 1);
     }
     __device__ __forceinline__ void init(const AttnArgs& a, const Plan& p, int lane) {
@@ -315,7 +323,7 @@ struct Line {
                 if (hi < longest && hi + p.piece_cost + p.join_cost < best) deal = kEven, per = hi;
             }
             if (deal != kLine) {
-                block(a, p, 0, lane);
+                weigh();
                 total = lane64(sum, 63);  // (kEven: one block of tiles)
             }
         }
@@ -327,14 +335,18 @@ struct Line {
         return (int)(((x + 1) * parts - 1) / total);
     }
 
-    // the tile at position x < total; positions of later calls do not decrease
+    // the tile at position x < total; positions of later calls do not decrease.  (steps = 0: there is none -- the lengths have
+    // changed under the call, which has to end all the same)
     __device__ __forceinline__ Piece find(const AttnArgs& a, const Plan& p, int64_t x, int lane) {
-        while (x >= before + lane64(sum, 63)) {
+        while (x >= before + lane64(sum, 63) && base + kWave < n_tiles) {
             before += lane64(sum, 63);
             block(a, p, base + kWave, lane);
         }
-        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(x < before + sum));
+        const uint64_t vote = __builtin_amdgcn_ballot_w64(x < before + sum);
         Piece r;
+        r.steps = 0;
+        if (vote == 0) return r;
+        const int at = __builtin_ctzll(vote);
         r.s = __builtin_amdgcn_readlane(s, at);
         r.tile = __builtin_amdgcn_readlane(t, at);
         r.q = Seq{__builtin_amdgcn_readlane(q.q0, at), __builtin_amdgcn_readlane(q.n, at),
@@ -372,6 +384,7 @@ __device__ __forceinline__ void for_each_piece(const AttnArgs& a, const Plan& p,
             line.block(a, p, (int)line.before, lane);
         }
         const Piece u = line.find(a, p, x, lane);
+        if (u.steps == 0) return;
         int from = 0, n = u.steps, pieces = 1, i0 = me, shift = 0;
         if (deal == kLine) {
             from = u.from;
@@ -386,6 +399,7 @@ __device__ __forceinline__ void for_each_piece(const AttnArgs& a, const Plan& p,
             n = (int)mul_div(u.steps, u.from + 1, pieces) - from;
             i0 = me - u.from;
         }
+        if (n < 1) return;
         if (pieces > 1 && x == begin && from > 0 && i0 == me - 1 && threadIdx.x == 0) {
             note[0] = pieces;
             note[1] = u.q.q0;

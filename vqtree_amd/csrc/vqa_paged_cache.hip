@@ -201,7 +201,7 @@ int read(const void* k_pages, const void* v_pages, const uint8_t* k_exp, const u
          const int32_t* lens, void* k, void* v, int S, int H, int n, int D, int page, int n_pages, int width, int e4m3,
          const int64_t* st, hipStream_t stream) {
     if (!k || !v || !k_pages || !v_pages || !table || !lens || !st) return VQA_ERR_NULL_POINTER;
-    if (H < 1 || H > 65535 || S > 65535 || n < 0) return VQA_ERR_BAD_SHAPE;
+    if (H < 1 || H > 65535 || S > 65535 || n < 0 || n > (1 << 30)) return VQA_ERR_BAD_SHAPE;
     if (D != 64 && D != 128) return VQA_ERR_UNSUPPORTED_HEAD_DIM;
     ReadArgs a{{}, {}, {}, (uint16_t*)k, (uint16_t*)v, st[11], st[12], st[13], st[14], st[15], st[16], n};
     if (int rc = make_seqs(&a.g, nullptr, lens, table, st[10], S, 0, width, n_pages, page)) return rc;
