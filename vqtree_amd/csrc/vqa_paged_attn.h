@@ -232,6 +232,9 @@ __device__ __forceinline__ int64_t mul_div(int64_t x, int i, int n) {
     return x * i / n;
 }
 
+// kWhole: which tile, counted from the last, is the j-th of part i -- there and back, so that the lengths even out
+__device__ __forceinline__ int whole_turn(int j, int i, int parts) { return j * parts + (j & 1 ? parts - 1 - i : i); }
+
 struct Piece {
     int s, tile;       // sequence, row tile
     Seq q;
@@ -308,10 +311,21 @@ struct Line {
                 block(a, p, 0, lane);
             }
             parts = total >= (int64_t)p.parts * p.min_steps ? p.parts : max(1, (int)total / p.min_steps);
-            // whole tiles, dealt out to all parts, take about as long as the longest one times the rounds
-            const int64_t whole = (int64_t)longest * ((n_tiles + p.parts - 1) / p.parts);
+            // whole tiles: the most that a part gets; beyond a wave of tiles, as if all were as long as the longest
+            const int rounds = (n_tiles + p.parts - 1) / p.parts;
+            int64_t whole = (int64_t)longest * rounds;
+            if (n_tiles <= kWave && rounds > 1) {
+                int load = 0;
+                for (int j = 0; j < rounds; ++j) {
+                    const int at = n_tiles - 1 - whole_turn(j, lane, p.parts);
+                    const int x = __shfl(steps, max(at, 0), 64);
+                    load += lane < p.parts && at >= 0 ? x : 0;
+                }
+                whole = wave_most(load);
+            }
+            whole += (rounds - 1) * p.piece_cost;
             const int64_t fair = mul_div(total, 1, parts);
-            int64_t best = fair + (n_tiles > 1 ? 2 : 1) * p.piece_cost + p.join_cost;
+            int64_t best = fair + (n_tiles > 1 ? 1 + rounds : 1) * p.piece_cost + p.join_cost;
             if (whole <= best) deal = kWhole, best = whole;
             if (p.even && n_tiles > 1 && n_tiles <= min(parts, kWave)) {
                 int lo = (int)fair, hi = longest;  // lo pieces: too many, hi: few enough
@@ -369,12 +383,13 @@ __device__ __forceinline__ void for_each_piece(const AttnArgs& a, const Plan& p,
     line.init(a, p, lane);
     const int deal = line.deal;
     int64_t x = 0, end = 0;
+    int turn = 0;
     if (deal == kLine) {
         if (me < line.parts) x = line.start(me), end = line.start(me + 1);
     } else if (deal == kEven) {
         x = me, end = min(line.total, (int64_t)me + 1);
     } else {
-        x = line.total - 1 - me;  // (downwards: the last ones first)
+        x = line.total - 1 - me;  // (downwards, the last and longest ones first)
     }
     if (deal == kWhole ? x < 0 : x >= end) return;
     const int64_t begin = x;
@@ -411,7 +426,7 @@ __device__ __forceinline__ void for_each_piece(const AttnArgs& a, const Plan& p,
         work(u, u.first + from, n, pieces == 1, 2 * me + (x == begin ? 0 : 1));
         if (deal == kLine) x += n;
         else if (deal == kEven) x += 1;
-        else x -= n_wgs;
+        else x = line.total - 1 - whole_turn(++turn, me, n_wgs);
         if (deal == kWhole ? x < 0 : x >= end) return;
         line.block(a, p, line.base, lane);
     }
