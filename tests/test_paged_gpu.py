@@ -26,6 +26,8 @@ DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
 class Cache:
     """A random cache on the CPU (pools, exponents, table, lengths) and its copy on the GPU."""
 
+    WIDE = False  # whether the tables have room for 2^18 keys more
+
     def __init__(self, new, past, *, Hkv=2, G=1, D=128, page=16, dtype=torch.bfloat16, e4m3=False, seed=0, extra=0,
                  spread=1.0):
         g = torch.Generator().manual_seed(seed)
@@ -33,7 +35,7 @@ class Cache:
         self.Hkv, self.G, self.D, self.page, self.dtype, self.e4m3 = Hkv, G, D, page, dtype, e4m3
         need = [-(-n // page) for n in self.lens]
         n_pages = sum(need) + 2 + extra
-        width = max(need + [1]) + 1
+        width = max(need + [1]) + 1 + (2**18 // page if Cache.WIDE else 0)
         order = torch.randperm(n_pages, generator=g).tolist()
         self.table = torch.full((len(new), width), -1, dtype=torch.int32)
         for s, n in enumerate(need):
@@ -95,6 +97,17 @@ def compare(got, want, c, rows=slice(None)):
         assert not bad.any(), f"lse: {int(bad.sum())} off, {float((lse - w_lse).abs().nan_to_num(0).max()):.3g}"
 
 
+@pytest.fixture(params=["table", "wide_table"])
+def table_width(request):
+    """Which kernel a call takes and how it is cut up follows from the room in the tables, so a test that uses this runs for
+    both: chunks of 65 rows and more with the few-rows kernel where the table ends behind the last page, and with their own."""
+    Cache.WIDE = request.param == "wide_table"
+    yield
+    Cache.WIDE = False
+
+
+both_widths = pytest.mark.usefixtures("table_width")
+
 FORMS = [("bf16", False, 128, 1, 16), ("bf16", True, 128, 4, 64), ("f16", False, 64, 4, 32), ("f16", True, 64, 1, 16),
          ("bf16", False, 128, 8, 64), ("bf16", True, 64, 7, 128), ("f16", True, 128, 2, 256)]
 LENGTHS = {
@@ -108,6 +121,7 @@ LENGTHS = {
 }
 
 
+@both_widths
 @pytest.mark.parametrize("form", FORMS, ids=lambda f: f"{f[0]}-{'e4m3' if f[1] else '16'}-d{f[2]}-g{f[3]}-p{f[4]}")
 @pytest.mark.parametrize("lengths", LENGTHS, ids=str)
 def test_attention(lengths, form):
@@ -133,10 +147,12 @@ DEALS = {  # new, past, Hkv, G, D, page: how the work is dealt out (few-rows ker
     "more_than_64_tiles": ([33, 70, 1] * 24, [i % 90 for i in range(72)], 1, 2, 64, 16),
     "long_tiles_beyond_64": ([70] * 66, [2100 + i for i in range(66)], 1, 1, 64, 256),
     "no_keys_at_all": ([100, 1], [0, 0], 2, 2, 64, 16),
+    "whole_tiles_in_turns": ([600], [0], 128, 1, 64, 16),
     "large_pages": ([65, 1], [5000, 4097], 2, 1, 64, 4096),
 }
 
 
+@both_widths
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("deal", DEALS, ids=str)
 def test_ways_of_dealing_out(deal, e4m3):
@@ -156,6 +172,7 @@ def test_ways_of_dealing_out(deal, e4m3):
         compare(got, want, c)
 
 
+@both_widths
 @pytest.mark.parametrize("new", [[1], [80]])
 def test_offsets_beyond_32_bits(new):
     """Pages that lie more than 4 GiB into the pools (and exponents far in): read, written and attended."""
@@ -186,6 +203,16 @@ def test_windows(window):
         c.check(window=window)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("window", [None, 0, 63, 129, 700])
+def test_long_chunks(window, e4m3):
+    c = Cache([1100, 2, 70], [300, 500, 0], Hkv=1, D=64, page=32, e4m3=e4m3, seed=24)
+    c.check(window=window, max_q_len=1100)
+    if window is None:
+        c.check(causal=False)
+
+
+@both_widths
 @pytest.mark.parametrize("scale", [1e-6, 1.0, 30.0])
 def test_scales(scale):
     """Flat, sharp and one-hot softmax: the tolerance is that of the scores the scale gives."""
@@ -300,6 +327,7 @@ def test_rows_that_have_no_place_are_skipped():
 
 # ---------------------------------------------------------------------------------------------------------------------
 # hidden places, missing pages, odd metadata
+@both_widths
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("new,past", [([1, 1], [20, 333]), ([130], [70]), ([300, 5], [0, 900])])
 def test_hidden_places_may_hold_anything(e4m3, new, past):
@@ -324,6 +352,7 @@ def test_hidden_places_may_hold_anything(e4m3, new, past):
     compare(c.attend(window=50, return_lse=True), clean, c)
 
 
+@both_widths
 @pytest.mark.parametrize("new", [7, 200])
 def test_a_later_tokens_nan_does_not_reach_earlier_rows(new):
     c = Cache([new], [90], D=64, page=16, G=2, seed=2)
@@ -336,6 +365,7 @@ def test_a_later_tokens_nan_does_not_reach_earlier_rows(new):
     assert torch.isinf(out[new - 3]).all() and torch.isnan(out[new - 2:]).all()
 
 
+@both_widths
 def test_missing_pages_and_odd_lengths():
     c = Cache([1, 40, 3, 2], [300, 100, 0, 700], D=128, page=16, G=2, seed=5)
     c.table[0, 3], c.table[0, 18], c.table[1, 0], c.table[3, 1] = -1, c.k.shape[0], 2**31 - 1, -(2**31)
@@ -356,6 +386,7 @@ def test_missing_pages_and_odd_lengths():
     compare(c.attend(return_lse=True), c.want(), c)
 
 
+@both_widths
 @pytest.mark.parametrize("new", [[1, 2], [90, 40]])
 def test_rows_behind_the_last_sequence_are_left_alone(new):
     c = Cache(new, [100, 30], D=64, G=4, seed=6)
@@ -367,6 +398,7 @@ def test_rows_behind_the_last_sequence_are_left_alone(new):
     compare((out[:T], lse[:T]), c.want(), c)
 
 
+@both_widths
 def test_numbers_out_of_range_do_no_harm():
     """cu_q that decreases or runs past the rows: memory stays in bounds; rows of well-formed sequences come out right."""
     c = Cache([4, 40, 4], [50, 20, 30], D=64, seed=7)
@@ -385,6 +417,7 @@ def test_numbers_out_of_range_do_no_harm():
 
 # ---------------------------------------------------------------------------------------------------------------------
 # layouts, streams, graphs, a whole run
+@both_widths
 @pytest.mark.parametrize("new", [[1, 1], [100, 3]])
 def test_strided_tensors(new):
     """q as columns of a projection, out as rows of a wider buffer, key and value pages interleaved in one pool."""
@@ -403,6 +436,7 @@ def test_strided_tensors(new):
     compare(P.attn_paged(qt, kv[:, 0], kv[:, 1], c.table.to(DEV), c.cu.to(DEV), c.kv_lens.to(DEV), return_lse=True), c.want(), c)
 
 
+@both_widths
 def test_another_stream_and_two_calls_at_once():
     a, b = Cache([1, 1], [3000, 700], seed=10, G=2), Cache([80], [900], seed=11, G=2, e4m3=True)
     sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
@@ -417,7 +451,7 @@ def test_another_stream_and_two_calls_at_once():
     compare(gots[1], b.want(), b)
 
 
-@pytest.mark.parametrize("width", [64, 400])
+@pytest.mark.parametrize("width", [64, 400, 2000])
 @pytest.mark.parametrize("new", [[1, 1, 1], [130, 1, 20]])
 def test_recorded_step_replays_on_new_lengths(new, width):
     """A whole step -- write, then attend -- recorded once: lengths, tables and rows change between the replays (and with

@@ -125,8 +125,26 @@ struct Cut {
 };
 
 constexpr int kCus = 256;           // workgroups that fill the chip: one per compute unit, in both kernels
-constexpr int kWholeSteps = 32;     // a tile of so few key steps is not worth a split and the launch that joins it
-constexpr int kFewRows = 64;        // sequences of more rows go to the chunk kernel
+
+// A tile of so few key steps is not worth a split and the launch that joins it: one token, 32 query and 8 key heads, whole /
+// split: 12.7 / 16.2 us for 1020 keys, 17.5 / 16.4 for 2000, 26.4 / 18.3 for 4000.  (Chunks of 2048 rows over 1500 keys: 53 /
+// 59.)
+constexpr int kWholeSteps = 32;
+
+// Sequences of more rows than this go to the chunk kernel, which reads the keys once for 256 rows where the few-rows kernel
+// does for 32, at a higher rate of products, but starts and ends slower: few / chunk, 32 new tokens for 4 x 8 heads (128 rows):
+// 32 sequences of 4096 keys 221 / 192 us, 8 of 2000 to 8300 keys 101 / 75; 16 new tokens (64 rows), one sequence of 4096 or
+// 32768 keys 21 / 29, 38 / 58.  Calls with little to do stay in the few-rows kernel up to kFewRowsSmall: tiles of 32 rows x key
+// heads x keys, as far as the host knows them, of at most kSmall.  128 rows, 8 sequences of 100 to 900 keys (0.2 M): 18 / 39;
+// 256 rows x 4096 keys (0.3 M): 26 / 38; 1024 rows x 1500 keys (0.4 M): 23 / 52; 512 rows x 4096 keys (0.5 M): 41 / 40; 512
+// rows, 8 sequences of 230 to 580 keys (0.6 M): 53 / 42; 256 rows x 32768 keys (2.1 M): 82 / 65.
+constexpr int kFewRows = 64, kFewRowsSmall = 1024;
+constexpr double kSmall = 1 << 19;
+
+// So many tiles are taken whole, one to a workgroup in the order of the grid, without a plan's search or a join.  Few rows: 512
+// tiles of 100 to 8000 keys are 181 us whole and 174 dealt out, 1024: 335 and 325, 2048: 637 and 639.  Chunks: between 1 and 8
+// times the compute units the time is the same within 3 %, as the plan takes tiles whole by itself where that is best.
+constexpr int kWholeTilesFew = 8 * kCus, kWholeTilesChunk = 4 * kCus;
 
 inline size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
 inline size_t o_bytes(const Plan& p, int Hkv, int D) { return round256((size_t)2 * p.parts * Hkv * p.rows * D * 4); }
@@ -139,7 +157,10 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
     Cut c{};
     const int64_t most = (int64_t)std::max(1, std::min(max_q, T)) * G;  // rows of a sequence
     const int64_t seqs = std::min(S, T), all = (int64_t)T * G;
-    const int limit = most > kFewRows ? kFewRows : 0x7fffffff;
+    const int64_t small = std::min<int64_t>(most, kFewRowsSmall);
+    const int64_t small_tiles = std::min(all / 32 + seqs, seqs * ((small + 31) / 32));
+    const int few_rows = (double)small_tiles * Hkv * keys <= kSmall ? kFewRowsSmall : kFewRows;
+    const int limit = most > few_rows ? few_rows : 0x7fffffff;
     const bool short_keys = keys <= (int64_t)kWholeSteps * kKeyStep;
     auto plan = [&](int rows, int lo, int hi, int whole_from, Plan& p, int64_t& grid, size_t& bytes) {
         const int64_t rows_each = std::min<int64_t>(most, hi);
@@ -150,10 +171,11 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
         bytes = o_bytes(p, Hkv, D) + ml_bytes(p, Hkv) + join_bytes(p, Hkv);
     };
     // (a hint that is too small keeps every sequence in the few-rows kernel; one that is too large costs an idle launch)
-    if (!(most > limit && S == 1 && max_q >= T && all > kFewRows))
+    if (!(most > limit && S == 1 && max_q >= T && all > few_rows))
         // (next to chunks most of the others are single tokens)
-        plan(std::min<int64_t>(most, limit) <= 16 || (most > limit && G <= 16) ? 16 : 32, 1, limit, 8 * kCus, c.few, c.few_grid, c.few_bytes);
-    if (most > limit) plan(256, limit + 1, 0x7fffffff, 4 * kCus, c.chunk, c.chunk_grid, c.chunk_bytes);
+        plan(std::min<int64_t>(most, limit) <= 16 || (most > limit && limit == kFewRows && G <= 16) ? 16 : 32, 1, limit,
+             kWholeTilesFew, c.few, c.few_grid, c.few_bytes);
+    if (most > limit) plan(256, limit + 1, 0x7fffffff, kWholeTilesChunk, c.chunk, c.chunk_grid, c.chunk_bytes);
     // in key steps of about 1 us (few rows) and 2 us (chunks)
     c.few.min_steps = 8, c.few.piece_cost = 2, c.few.join_cost = 2, c.few.even = 0;
     c.chunk.min_steps = 4, c.chunk.piece_cost = 8, c.chunk.join_cost = 10, c.chunk.even = 1;
