@@ -135,11 +135,16 @@ constexpr int kWholeSteps = 32;
 // does for 32, at a higher rate of products, but starts and ends slower: few / chunk, 32 new tokens for 4 x 8 heads (128 rows):
 // 32 sequences of 4096 keys 221 / 192 us, 8 of 2000 to 8300 keys 101 / 75; 16 new tokens (64 rows), one sequence of 4096 or
 // 32768 keys 21 / 29, 38 / 58.  Calls with little to do stay in the few-rows kernel up to kFewRowsSmall: tiles of 32 rows x key
-// heads x keys, as far as the host knows them, of at most kSmall.  128 rows, 8 sequences of 100 to 900 keys (0.2 M): 18 / 39;
+// heads x keys, as far as the host knows them, below kSmall.  128 rows, 8 sequences of 100 to 900 keys (0.2 M): 18 / 39;
 // 256 rows x 4096 keys (0.3 M): 26 / 38; 1024 rows x 1500 keys (0.4 M): 23 / 52; 512 rows x 4096 keys (0.5 M): 41 / 40; 512
 // rows, 8 sequences of 230 to 580 keys (0.6 M): 53 / 42; 256 rows x 32768 keys (2.1 M): 82 / 65.
 constexpr int kFewRows = 64, kFewRowsSmall = 1024;
 constexpr double kSmall = 1 << 19;
+
+// The few-rows kernel's tiles have 16 rows where that is all there are (one token / 16 sequences of it, 4 x 8 heads, 16 rows
+// against 32: 12.9 / 15.8, 193 / 223 us), and where a workgroup is left for each of them and little to read twice: 20 rows of 8
+// sequences 12.1 / 14.4, 64 rows of 8 short sequences 13.8 / 17.0, 512 rows x 128 keys 9.4 / 11.5, x 1500 keys 17.6 / 21.2; but
+// 1024 rows x 256 keys (512 tiles of 16) 17.2 / 12.2, 64 rows x 32768 keys 54 / 38, 32 sequences of 64 rows x 4096 222 / 118.
 
 // So many tiles are taken whole, one to a workgroup in the order of the grid, without a plan's search or a join.  Few rows: 512
 // tiles of 100 to 8000 keys are 181 us whole and 174 dealt out, 1024: 335 and 325, 2048: 637 and 639.  Chunks: between 1 and 8
@@ -157,26 +162,30 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
     Cut c{};
     const int64_t most = (int64_t)std::max(1, std::min(max_q, T)) * G;  // rows of a sequence
     const int64_t seqs = std::min(S, T), all = (int64_t)T * G;
-    const int64_t small = std::min<int64_t>(most, kFewRowsSmall);
-    const int64_t small_tiles = std::min(all / 32 + seqs, seqs * ((small + 31) / 32));
-    const int few_rows = (double)small_tiles * Hkv * keys <= kSmall ? kFewRowsSmall : kFewRows;
+    auto tiles_of = [&](int rows, int64_t rows_each) {  // at most, over all sequences
+        return std::min(all / rows + seqs, seqs * ((rows_each + rows - 1) / rows));
+    };
+    auto little = [&](int64_t tiles) { return (double)tiles * Hkv * keys < kSmall; };
+    const int few_rows = little(tiles_of(32, std::min<int64_t>(most, kFewRowsSmall))) ? kFewRowsSmall : kFewRows;
     const int limit = most > few_rows ? few_rows : 0x7fffffff;
     const bool short_keys = keys <= (int64_t)kWholeSteps * kKeyStep;
     auto plan = [&](int rows, int lo, int hi, int whole_from, Plan& p, int64_t& grid, size_t& bytes) {
-        const int64_t rows_each = std::min<int64_t>(most, hi);
-        const int64_t tiles = std::min(all / rows + seqs, seqs * ((rows_each + rows - 1) / rows));
+        const int64_t tiles = tiles_of(rows, std::min<int64_t>(most, hi));
         p.rows = rows, p.lo = lo, p.hi = hi;
         p.parts = tiles * Hkv >= whole_from || short_keys ? 0 : std::max(1, kCus / Hkv);
         grid = (p.parts ? p.parts : tiles) * Hkv;
         bytes = o_bytes(p, Hkv, D) + ml_bytes(p, Hkv) + join_bytes(p, Hkv);
     };
     // (a hint that is too small keeps every sequence in the few-rows kernel; one that is too large costs an idle launch)
-    if (!(most > limit && S == 1 && max_q >= T && all > few_rows))
+    if (!(most > limit && S == 1 && max_q >= T && all > few_rows)) {
+        const int64_t rows_each = std::min<int64_t>(most, limit), tiles16 = tiles_of(16, rows_each);
         // (next to chunks most of the others are single tokens)
-        plan(std::min<int64_t>(most, limit) <= 16 || (most > limit && limit == kFewRows && G <= 16) ? 16 : 32, 1, limit,
-             kWholeTilesFew, c.few, c.few_grid, c.few_bytes);
+        const bool rows16 = rows_each <= 16 || (tiles16 * Hkv <= kCus && little(tiles16)) || (limit == kFewRows && G <= 16);
+        plan(rows16 ? 16 : 32, 1, limit, kWholeTilesFew, c.few, c.few_grid, c.few_bytes);
+    }
     if (most > limit) plan(256, limit + 1, 0x7fffffff, kWholeTilesChunk, c.chunk, c.chunk_grid, c.chunk_bytes);
-    // in key steps of about 1 us (few rows) and 2 us (chunks)
+    // In key steps of about 1 us (few rows) and 2 us (chunks).  Equal pieces beside the line, chunks: 2048 rows x 4096 keys 62 us
+    // with and 74 without, 32 sequences of 128 rows x 4096 keys 177 and 191, where all units are busy anyway no difference; few rows: none.
     c.few.min_steps = 8, c.few.piece_cost = 2, c.few.join_cost = 2, c.few.even = 0;
     c.chunk.min_steps = 4, c.chunk.piece_cost = 8, c.chunk.join_cost = 10, c.chunk.even = 1;
     return c;
