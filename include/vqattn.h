@@ -8,9 +8,9 @@
  *     vqa_decode_static_bf16, works in a fixed device array of the library and says so below).  What the library does
  *     remember, behind a mutex, is per-device set-up done on first use: the raised dynamic-LDS limit of the kernels
  *     that need more than 64 KB (the count kernel at head dim 128, the pipelined prefill / window kernels, the paged
- *     attention) and the
- *     device address of that array.  Both belong to the device that owns the call's operands, which must be the
- *     calling thread's current device (VQA_ERR_BAD_ARGUMENT otherwise: the kernels would be launched elsewhere),
+ *     attention) and the device address of that array.  Both belong to the device that owns the call's operands, which
+ *     must be the calling thread's current device (VQA_ERR_BAD_ARGUMENT otherwise: the kernels would be launched
+ *     elsewhere),
  *   - returns VQA_OK (0) or a negative vqa_status; it never throws or aborts.
  * Tensors are addressed as base + sum(index_i * stride_i) in ELEMENTS of their own type; the innermost
  * (head_dim / codebook index M) stride must be 1.  Head dims of the attention entry points: 64 and 128; vqa_local_attn_*,

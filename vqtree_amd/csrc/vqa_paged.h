@@ -44,18 +44,6 @@ __device__ __forceinline__ Seq seq_of(const Seqs& g, int s) {
     return r;
 }
 
-// number of sequences that end at or before packed row t: the sequence of row t (S: behind the last one).  The whole wave
-// counts, so a batch of 64 sequences costs one load.
-__device__ __forceinline__ int find_seq(const Seqs& g, int t, int lane) {
-    int s = 0;
-    for (int base = 0; base < g.S; base += kWave) {
-        const int i = base + lane;
-        const bool before = i < g.S && g.cu[i + 1] <= t;
-        s += __popcll(__builtin_amdgcn_ballot_w64(before));
-    }
-    return s;
-}
-
 // page of row j (0 <= j < width << page_shift) of sequence s, -1 if it is not there
 __device__ __forceinline__ int page_of(const Seqs& g, int s, int j) {
     const int page = g.table[(int64_t)s * g.table_ss + (j >> g.page_shift)];

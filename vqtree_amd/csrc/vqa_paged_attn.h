@@ -149,10 +149,11 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& 
 // r / G, head r % G of the group), cut into tiles; a tile has as many key steps (64 keys) as its rows see.  The lengths are
 // known on the device only, so that is where the work of a key head is dealt out to its workgroups ("parts"), in one of three
 // ways, whichever ends first by the counts of steps and what a piece of a tile costs:
-//   kWhole  whole tiles, the last (longest) ones of the sequences first;
+//   kWhole  whole tiles, the last (longest) ones of the sequences first, in turns there and back over the parts;
 //   kEven   every tile in equal pieces, one piece to a part: the shortest pieces that give no more of them than parts;
 //   kLine   the steps of all tiles stand in one line and every part takes an equal stretch of it, wherever tiles begin and
 //           end: perfect balance however unequal the lengths, at the price of two or more pieces in a part.
+// (A prompt of 4096 tokens, 32 heads, on 8 parts a head: 190 us in whole tiles, 258 in a line.)
 // A piece that is not a whole tile leaves an unnormalised result, which join_kernel puts together.  Every workgroup computes
 // the same plan from the same numbers, and so does a recorded call that is replayed on new ones.
 // ---------------------------------------------------------------------------------------------------------------------

@@ -1,6 +1,9 @@
 // Few rows, many keys: generation steps, drafted tokens, short chunks (vqa_paged_attn_*).  HBM bound: every key and value
 // row of a (sequence, key head) is read once for all rows of a tile, 16 * NB of them (grouped query heads and new tokens
-// together).
+// together).  Measured (kernel time): 16 sequences, 260 000 keys together, 32 query and 8 key heads, head dim 128: 185 us for
+// 1.19 GB of 16-bit rows, 6.4 TB/s (reads alone reach about 7); 65 536 keys of 32 heads in e4m3: 92 us for 0.54 GB, 5.9 TB/s.
+// One sequence of 1000 keys is latency: 12.5 us -- 2 until the work is dealt out, 1 until the first tile is asked for, 4 for
+// four tiles per wave, 3 to join the waves.
 //
 // One workgroup works on one piece of a tile's keys at a time; its waves take consecutive parts of it and never wait for
 // each other until their results are joined at the end.  A wave walks 32-key tiles: the rows go HBM -> LDS directly
