@@ -148,6 +148,8 @@ DEALS = {  # new, past, Hkv, G, D, page: how the work is dealt out (few-rows ker
     "long_tiles_beyond_64": ([70] * 66, [2100 + i for i in range(66)], 1, 1, 64, 256),
     "no_keys_at_all": ([100, 1], [0, 0], 2, 2, 64, 16),
     "whole_tiles_in_turns": ([600], [0], 128, 1, 64, 16),
+    "many_short_tiles_of_32_rows": ([150, 3, 40], [0, 30, 64], 32, 2, 128, 16),
+    "many_single_tokens": ([1] * 12, [7 * i * i for i in range(12)], 32, 1, 128, 16),
     "large_pages": ([65, 1], [5000, 4097], 2, 1, 64, 4096),
 }
 

@@ -161,6 +161,7 @@ constexpr int kKeyStep = 64;
 
 struct Plan {
     int rows;       // rows of a tile (a power of two)
+    int waves;      // of a workgroup (few-rows kernel)
     int lo, hi;     // sequences with lo <= n * G <= hi belong to this kernel
     int parts;      // workgroups per key head; 0: no pieces, the grid has a workgroup for every tile there may be
     int min_steps;  // fewest steps worth a workgroup

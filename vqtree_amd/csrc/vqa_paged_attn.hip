@@ -134,11 +134,11 @@ constexpr int kWholeSteps = 32;
 // Sequences of more rows than this go to the chunk kernel, which reads the keys once for 256 rows where the few-rows kernel
 // does for 32, at a higher rate of products, but starts and ends slower: few / chunk, 32 new tokens for 4 x 8 heads (128 rows):
 // 32 sequences of 4096 keys 221 / 192 us, 8 of 2000 to 8300 keys 101 / 75; 16 new tokens (64 rows), one sequence of 4096 or
-// 32768 keys 21 / 29, 38 / 58.  Calls with little to do stay in the few-rows kernel up to kFewRowsSmall: tiles of 32 rows x key
-// heads x keys, as far as the host knows them, below kSmall.  128 rows, 8 sequences of 100 to 900 keys (0.2 M): 18 / 39;
+// 32768 keys 21 / 29, 38 / 58.  Calls with little to do stay in the few-rows kernel: tiles of 32 rows x key heads
+// x keys, as far as the host knows them, below kSmall.  128 rows, 8 sequences of 100 to 900 keys (0.2 M): 18 / 39;
 // 256 rows x 4096 keys (0.3 M): 26 / 38; 1024 rows x 1500 keys (0.4 M): 23 / 52; 512 rows x 4096 keys (0.5 M): 41 / 40; 512
 // rows, 8 sequences of 230 to 580 keys (0.6 M): 53 / 42; 256 rows x 32768 keys (2.1 M): 82 / 65.
-constexpr int kFewRows = 64, kFewRowsSmall = 1024;
+constexpr int kFewRows = 64;
 constexpr double kSmall = 1 << 19;
 
 // The few-rows kernel's tiles have 16 rows where that is all there are (one token / 16 sequences of it, 4 x 8 heads, 16 rows
@@ -150,6 +150,11 @@ constexpr double kSmall = 1 << 19;
 // tiles of 100 to 8000 keys are 181 us whole and 174 dealt out, 1024: 335 and 325, 2048: 637 and 639.  Chunks: between 1 and 8
 // times the compute units the time is the same within 3 %, as the plan takes tiles whole by itself where that is best.
 constexpr int kWholeTilesFew = 8 * kCus, kWholeTilesChunk = 4 * kCus;
+
+// Workgroups of the few-rows kernel have 8 waves; 4, two to a compute unit, where whole tiles are more than the units.  43
+// sequences of 16 to 855 keys, 32 heads: 54 / 69 us with 4 / 8 waves, e4m3 and head dim 64 34 / 52; 403 tokens of 4 x 8 heads
+// 13.4 / 22; 16 sequences up to 32 768 keys 192 / 193, but one sequence of 1000 keys 15.8 / 12.9, 65 536 in e4m3 126 / 97.
+constexpr int kManyWaves = 8, kFewWaves = 4;
 
 inline size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
 inline size_t o_bytes(const Plan& p, int Hkv, int D) { return round256((size_t)2 * p.parts * Hkv * p.rows * D * 4); }
@@ -166,8 +171,7 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
         return std::min(all / rows + seqs, seqs * ((rows_each + rows - 1) / rows));
     };
     auto little = [&](int64_t tiles) { return (double)tiles * Hkv * keys < kSmall; };
-    const int few_rows = little(tiles_of(32, std::min<int64_t>(most, kFewRowsSmall))) ? kFewRowsSmall : kFewRows;
-    const int limit = most > few_rows ? few_rows : 0x7fffffff;
+    const int limit = most <= kFewRows || little(tiles_of(32, most)) ? 0x7fffffff : kFewRows;
     const bool short_keys = keys <= (int64_t)kWholeSteps * kKeyStep;
     auto plan = [&](int rows, int lo, int hi, int whole_from, Plan& p, int64_t& grid, size_t& bytes) {
         const int64_t tiles = tiles_of(rows, std::min<int64_t>(most, hi));
@@ -177,11 +181,11 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
         bytes = o_bytes(p, Hkv, D) + ml_bytes(p, Hkv) + join_bytes(p, Hkv);
     };
     // (a hint that is too small keeps every sequence in the few-rows kernel; one that is too large costs an idle launch)
-    if (!(most > limit && S == 1 && max_q >= T && all > few_rows)) {
+    if (!(most > limit && S == 1 && max_q >= T && all > kFewRows)) {
         const int64_t rows_each = std::min<int64_t>(most, limit), tiles16 = tiles_of(16, rows_each);
-        // (next to chunks most of the others are single tokens)
-        const bool rows16 = rows_each <= 16 || (tiles16 * Hkv <= kCus && little(tiles16)) || (limit == kFewRows && G <= 16);
+        const bool rows16 = rows_each <= 16 || (tiles16 * Hkv <= kCus && little(tiles16));
         plan(rows16 ? 16 : 32, 1, limit, kWholeTilesFew, c.few, c.few_grid, c.few_bytes);
+        c.few.waves = c.few.parts == 0 && c.few_grid > kCus ? kFewWaves : kManyWaves;
     }
     if (most > limit) plan(256, limit + 1, 0x7fffffff, kWholeTilesChunk, c.chunk, c.chunk_grid, c.chunk_bytes);
     // In key steps of about 1 us (few rows) and 2 us (chunks).  Equal pieces beside the line, chunks: 2048 rows x 4096 keys 62 us

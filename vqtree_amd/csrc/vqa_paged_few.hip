@@ -5,7 +5,8 @@
 // One sequence of 1000 keys is latency: 12.5 us -- 2 until the work is dealt out, 1 until the first tile is asked for, 4 for
 // four tiles per wave, 3 to join the waves.
 //
-// One workgroup works on one piece of a tile's keys at a time; its waves take consecutive parts of it and never wait for
+// One workgroup of 8 waves, or 4 where there are enough tiles for two workgroups on a compute unit (the start and the end of one
+// under the loads of the other), works on one piece of a tile's keys at a time; its waves take consecutive parts of it and never wait for
 // each other until their results are joined at the end.  A wave walks 32-key tiles: the rows go HBM -> LDS directly
 // (global_load_lds_dwordx4, whole rows per instruction, no registers), S^T = K.Q^T and O^T = V^T.P^T run on
 // v_mfma_f32_16x16x32 -- the matrix pipe has room to spare at any memory rate, so a single query row goes through it too.
@@ -33,7 +34,6 @@ using flash::u32x4_t;
 typedef flash::s16x4_t s16x4_t;
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 8;
 constexpr int kKeys = 32;    // keys per tile
 constexpr float kLazy = 8.f; // a row's reference maximum moves when a tile exceeds it by 2^kLazy
 
@@ -84,7 +84,7 @@ __device__ __forceinline__ float quads_sum(float x) {
 
 // Brings tiles of one wave.  kOnce: no other tile reads these rows (all rows of a sequence fit one tile), so the loads are
 // marked non-temporal: 213 -> 189 us for 1.19 GB of 16-bit rows, 105 -> 95 us for 0.54 GB of e4m3 rows.
-template <int D, bool kE4m3, bool kOnce>
+template <int D, bool kE4m3>
 struct Loader {
     typedef Geo<D, kE4m3> G;
     const char *k, *v;             // pools at the key head
@@ -146,7 +146,7 @@ struct Loader {
         }
         return x;
     }
-    template <bool kV>
+    template <bool kV, bool kOnce>
     __device__ __forceinline__ void request(const AttnArgs& a, const Place& x, int slot) {
         const uint32_t dst = lds + (uint32_t)(slot * G::kSlot) + (kV ? G::kTile : 0);
         const Pool& pool = kV ? a.vp : a.kp;
@@ -158,14 +158,14 @@ struct Loader {
         if (x.j[1] + 16 <= end && x.j[0] != x.j[1]) {
             flash2::static_for<G::kLoads>([&](auto I) {
                 constexpr int i = decltype(I)::value;
-                issue<i>(dst, kV ? v_off[i] : k_off[i], group[i * G::kRowsPerLoad / 16]);
+                issue<i, kOnce>(dst, kV ? v_off[i] : k_off[i], group[i * G::kRowsPerLoad / 16]);
             });
         } else {
             flash2::static_for<G::kLoads>([&](auto I) {
                 constexpr int i = decltype(I)::value;
                 constexpr int gi = i * G::kRowsPerLoad / 16;
                 const uint32_t row = (uint32_t)min(row_of_load(i, lane), end - 1 - x.j[gi]);
-                issue<i>(dst, row * (uint32_t)pool.sn + piece_of<kV>(i, lane), group[gi]);
+                issue<i, kOnce>(dst, row * (uint32_t)pool.sn + piece_of<kV>(i, lane), group[gi]);
             });
         }
         if constexpr (kE4m3 && !kV) {
@@ -178,7 +178,7 @@ struct Loader {
             }
         }
     }
-    template <int I>
+    template <int I, bool kOnce>
     static __device__ __forceinline__ void issue(uint32_t dst, uint32_t off, const char* base) {
         // (a load may not follow the write of M0 directly)
         if constexpr (kOnce)
@@ -194,14 +194,16 @@ struct Loader {
     }
 };
 
-template <typename Tag, int D, bool kE4m3, int NB>
-__global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
+// kBlocks: rows of a tile in blocks of 16.  In tiles of two a sequence that has one is done as one, so single tokens do not pay
+// for the drafts and short chunks they share a call with (generation step of 16 sequences: two blocks 223 us, one 193).
+template <typename Tag, int D, bool kE4m3, int kBlocks, int kWaves>
+__global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(AttnArgs a, Plan p) {
     typedef Geo<D, kE4m3> G;
     typedef typename Elem<Tag>::vec8 vec8;
     typedef typename std::conditional<kE4m3, bf16_tag, Tag>::type PTag;  // element type of the P.V product
     typedef typename Elem<PTag>::vec8 pvec8;
     constexpr bool kSplitP = std::is_same<PTag, bf16_tag>::value;
-    constexpr int kRows = 16 * NB;
+    constexpr int kTileRows = 16 * kBlocks;
     constexpr int kStageRow = D + 4;  // floats; the padding spreads a column of rows over the banks
     typedef const __attribute__((address_space(3))) u32x4_t* lds16_ptr;
     typedef __attribute__((address_space(3))) s16x4_t* lds_tr_ptr;
@@ -215,13 +217,15 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
     const int n = lane & 15, quad = lane >> 4;
     const int h = __builtin_amdgcn_readfirstlane((int)(blockIdx.x % (unsigned)a.Hkv));
     const uint32_t lds0 = flash::lds_addr_of(smem);
-    Loader<D, kE4m3, NB == 1> ld;
+    Loader<D, kE4m3> ld;
     ld.init(a, h, lds0 + (uint32_t)(wave * G::kWaveBytes), lane);
 
-    for_each_piece(a, p, lane,
-                   [&](const Piece& u, int step, int n_steps, bool whole, int slot_out) __attribute__((always_inline)) {
+    auto piece = [&](auto blocks, const Piece& u, int step, int n_steps, bool whole, int slot_out) __attribute__((always_inline)) {
+        constexpr int NB = decltype(blocks)::value, kRows = 16 * NB;
+        constexpr bool kOnce = NB == 1;
         const Seq& q = u.q;
-        const int n_rows = min(kRows, q.n * a.G - u.tile * kRows);  // (a tile is of one sequence: fits 32 bits)
+        const int row0 = u.tile * kTileRows;
+        const int n_rows = min(kRows, q.n * a.G - row0);  // (a tile is of one sequence: fits 32 bits)
         const int u_lo = step * kKeyStep;
         const int u_hi = (int)min((int64_t)(step + n_steps) * kKeyStep, (int64_t)q.keys);
         // this wave's part, in tiles
@@ -229,12 +233,12 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
         const int t_lo = n_tiles * wave / kWaves, t_hi = n_tiles * (wave + 1) / kWaves;
 
         ld.sequence(a, u.s, u_hi);
-        typename Loader<D, kE4m3, NB == 1>::Place places[G::kRing];
+        typename Loader<D, kE4m3>::Place places[G::kRing];
         auto ask_k = [&](int t, int slot) __attribute__((always_inline)) {
             places[slot] = ld.place(a.g, u_lo + t * kKeys);
-            ld.template request<false>(a, places[slot], slot);
+            ld.template request<false, kOnce>(a, places[slot], slot);
         };
-        auto ask_v = [&](int slot) __attribute__((always_inline)) { ld.template request<true>(a, places[slot], slot); };
+        auto ask_v = [&](int slot) __attribute__((always_inline)) { ld.template request<true, kOnce>(a, places[slot], slot); };
 #pragma unroll
         for (int i = 0; i < G::kRing; ++i)
             if (t_lo + i < t_hi) ask_k(t_lo + i, i), ask_v(i);
@@ -245,7 +249,7 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
         int all_lo = 0, all_hi = 0x7fffffff;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const int r = u.tile * kRows + min(b * 16 + n, n_rows - 1);
+            const int r = row0 + min(b * 16 + n, n_rows - 1);
             const int t = r / a.G, g = r - t * a.G;
             const Range v = visible(a, q, t);
             lo[b] = v.lo, hi[b] = v.hi;
@@ -257,7 +261,7 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
             }
         }
         {   // what every row of the tile sees: the first row's end and the last row's start
-            const int t0 = u.tile * kRows / a.G, t1 = (u.tile * kRows + n_rows - 1) / a.G;
+            const int t0 = row0 / a.G, t1 = (row0 + n_rows - 1) / a.G;
             all_hi = visible(a, q, t0).hi, all_lo = visible(a, q, t1).lo;
         }
 
@@ -439,7 +443,7 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
         }
         __syncthreads();
         constexpr int kLanes = D / 8;  // threads per row, 8 elements each
-        const int64_t part = ((int64_t)slot_out * a.Hkv + h) * kRows;
+        const int64_t part = ((int64_t)slot_out * a.Hkv + h) * kTileRows;
 #pragma unroll
         for (int i = 0; i < kRows * kLanes / (kWaves * 64) + (kRows * kLanes % (kWaves * 64) ? 1 : 0); ++i) {
             const int at = i * kWaves * 64 + (int)threadIdx.x;
@@ -470,7 +474,7 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
                 }
             } else {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const int rr = u.tile * kRows + r, t = rr / a.G, hq = h * a.G + rr - t * a.G;
+                const int rr = row0 + r, t = rr / a.G, hq = h * a.G + rr - t * a.G;
                 const u32x4_t pk = {Elem<Tag>::pack2(v[0] * inv, v[1] * inv), Elem<Tag>::pack2(v[2] * inv, v[3] * inv),
                                     Elem<Tag>::pack2(v[4] * inv, v[5] * inv), Elem<Tag>::pack2(v[6] * inv, v[7] * inv)};
                 *reinterpret_cast<u32x4_t*>(a.out + (int64_t)(q.q0 + t) * a.o_st + (int64_t)hq * a.o_sh + c * 8) = pk;
@@ -483,7 +487,7 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
         uint64_t todo = *bad;
         for (int r = 0; todo; ++r, todo >>= 1) {
             if (!(todo & 1) || r % kWaves != wave) continue;
-            const int rr = u.tile * kRows + r, t = rr / a.G, hq = h * a.G + rr - t * a.G;
+            const int rr = row0 + r, t = rr / a.G, hq = h * a.G + rr - t * a.G;
             const Range v = visible(a, q, t);
             RowState<D> st;
             row_by_lanes<Tag, D, kE4m3>(a, u.s, h, a.q + (int64_t)(q.q0 + t) * a.q_st + (int64_t)hq * a.q_sh, max(u_lo, v.lo),
@@ -500,37 +504,47 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(AttnArgs a, Plan p) {
             }
         }
         __syncthreads();  // the staging area is free for the next piece's tiles
+    };
+    for_each_piece(a, p, lane,
+                   [&](const Piece& u, int step, int n_steps, bool whole, int slot_out) __attribute__((always_inline)) {
+        if (kBlocks == 1 || u.q.n * a.G <= 16)
+            piece(std::integral_constant<int, 1>(), u, step, n_steps, whole, slot_out);
+        else
+            piece(std::integral_constant<int, kBlocks>(), u, step, n_steps, whole, slot_out);
     });
 }
 
-template <int D, bool kE4m3, int NB>
+template <int D, bool kE4m3, int NB, int kWaves>
 constexpr int lds_bytes() {
     const int tiles = kWaves * Geo<D, kE4m3>::kWaveBytes;
     const int join = kWaves * 16 * NB * (D + 4) * 4 + kWaves * 16 * NB * 8 + 16;
     return tiles > join ? tiles : join;
 }
 
-template <typename Tag, int D, bool kE4m3, int NB>
+template <typename Tag, int D, bool kE4m3, int NB, int kWaves>
 int launch(const AttnArgs& a, const Plan& p, int64_t grid, hipStream_t stream) {
-    constexpr int bytes = lds_bytes<D, kE4m3, NB>();
+    constexpr int bytes = lds_bytes<D, kE4m3, NB, kWaves>();
     if (bytes > 64 * 1024) {
-        if (int rc = raise_lds<few_kernel<Tag, D, kE4m3, NB>>(a.q, bytes)) return rc;
+        if (int rc = raise_lds<few_kernel<Tag, D, kE4m3, NB, kWaves>>(a.q, bytes)) return rc;
     }
-    few_kernel<Tag, D, kE4m3, NB><<<dim3((unsigned)grid), kWaves * 64, bytes, stream>>>(a, p);
+    few_kernel<Tag, D, kE4m3, NB, kWaves><<<dim3((unsigned)grid), kWaves * 64, bytes, stream>>>(a, p);
     return launch_status();
+}
+
+template <typename Tag, int D, bool kE4m3>
+int launch(const AttnArgs& a, const Plan& p, int64_t grid, hipStream_t stream) {
+    if (p.waves == 4)
+        return p.rows == 32 ? launch<Tag, D, kE4m3, 2, 4>(a, p, grid, stream) : launch<Tag, D, kE4m3, 1, 4>(a, p, grid, stream);
+    return p.rows == 32 ? launch<Tag, D, kE4m3, 2, 8>(a, p, grid, stream) : launch<Tag, D, kE4m3, 1, 8>(a, p, grid, stream);
 }
 
 }  // namespace few
 
 template <typename Tag>
 int launch_few(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream) {
-    const bool two = p.rows == 32;
-    if (D == 128) {
-        if (e4m3) return two ? few::launch<Tag, 128, true, 2>(a, p, grid, stream) : few::launch<Tag, 128, true, 1>(a, p, grid, stream);
-        return two ? few::launch<Tag, 128, false, 2>(a, p, grid, stream) : few::launch<Tag, 128, false, 1>(a, p, grid, stream);
-    }
-    if (e4m3) return two ? few::launch<Tag, 64, true, 2>(a, p, grid, stream) : few::launch<Tag, 64, true, 1>(a, p, grid, stream);
-    return two ? few::launch<Tag, 64, false, 2>(a, p, grid, stream) : few::launch<Tag, 64, false, 1>(a, p, grid, stream);
+    if (D == 128)
+        return e4m3 ? few::launch<Tag, 128, true>(a, p, grid, stream) : few::launch<Tag, 128, false>(a, p, grid, stream);
+    return e4m3 ? few::launch<Tag, 64, true>(a, p, grid, stream) : few::launch<Tag, 64, false>(a, p, grid, stream);
 }
 template int launch_few<bf16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);
 template int launch_few<f16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);
