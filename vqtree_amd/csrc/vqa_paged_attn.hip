@@ -134,17 +134,19 @@ constexpr int kWholeSteps = 32;
 // Sequences of more rows than this go to the chunk kernel, which reads the keys once for 256 rows where the few-rows kernel
 // does for 32, at a higher rate of products, but starts and ends slower: few / chunk, 32 new tokens for 4 x 8 heads (128 rows):
 // 32 sequences of 4096 keys 221 / 192 us, 8 of 2000 to 8300 keys 101 / 75; 16 new tokens (64 rows), one sequence of 4096 or
-// 32768 keys 21 / 29, 38 / 58.  Calls with little to do stay in the few-rows kernel: tiles of 32 rows x key heads
-// x keys, as far as the host knows them, below kSmall.  128 rows, 8 sequences of 100 to 900 keys (0.2 M): 18 / 39;
-// 256 rows x 4096 keys (0.3 M): 26 / 38; 1024 rows x 1500 keys (0.4 M): 23 / 52; 512 rows x 4096 keys (0.5 M): 41 / 40; 512
-// rows, 8 sequences of 230 to 580 keys (0.6 M): 53 / 42; 256 rows x 32768 keys (2.1 M): 82 / 65.
+// 32768 keys 21 / 29, 38 / 58.  Calls with little to do stay in the few-rows kernel: tiles of 32 rows x key heads x keys, as far
+// as the host knows them, below kSmall.  128 rows, 8 sequences of 100 to 900 keys (0.2 M): 18 / 39; 256 rows x 4096 keys (0.3 M):
+// 26 / 38; 1024 rows x 1500 keys (0.4 M): 23 / 52; 512 rows, 8 sequences of 230 to 580 keys (0.6 M): 33 / 41; 2048 rows x 1500
+// keys (0.8 M): 32 / 53; 128 rows x 32768 keys (1.0 M): 51 / 60; 1024 rows, 8 sequences of 360 to 710 keys (1.5 M): 68 / 47; 256
+// rows x 32768 keys (2.1 M): 83 / 65.
 constexpr int kFewRows = 64;
-constexpr double kSmall = 1 << 19;
+constexpr double kSmall = 5 << 18;
 
 // The few-rows kernel's tiles have 16 rows where that is all there are (one token / 16 sequences of it, 4 x 8 heads, 16 rows
 // against 32: 12.9 / 15.8, 193 / 223 us), and where a workgroup is left for each of them and little to read twice: 20 rows of 8
 // sequences 12.1 / 14.4, 64 rows of 8 short sequences 13.8 / 17.0, 512 rows x 128 keys 9.4 / 11.5, x 1500 keys 17.6 / 21.2; but
 // 1024 rows x 256 keys (512 tiles of 16) 17.2 / 12.2, 64 rows x 32768 keys 54 / 38, 32 sequences of 64 rows x 4096 222 / 118.
+constexpr double kSmall16 = 1 << 19;
 
 // So many tiles are taken whole, one to a workgroup in the order of the grid, without a plan's search or a join.  Few rows: 512
 // tiles of 100 to 8000 keys are 181 us whole and 174 dealt out, 1024: 335 and 325, 2048: 637 and 639.  Chunks: between 1 and 8
@@ -170,8 +172,7 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
     auto tiles_of = [&](int rows, int64_t rows_each) {  // at most, over all sequences
         return std::min(all / rows + seqs, seqs * ((rows_each + rows - 1) / rows));
     };
-    auto little = [&](int64_t tiles) { return (double)tiles * Hkv * keys < kSmall; };
-    const int limit = most <= kFewRows || little(tiles_of(32, most)) ? 0x7fffffff : kFewRows;
+    const int limit = most <= kFewRows || (double)tiles_of(32, most) * Hkv * keys < kSmall ? 0x7fffffff : kFewRows;
     const bool short_keys = keys <= (int64_t)kWholeSteps * kKeyStep;
     auto plan = [&](int rows, int lo, int hi, int whole_from, Plan& p, int64_t& grid, size_t& bytes) {
         const int64_t tiles = tiles_of(rows, std::min<int64_t>(most, hi));
@@ -183,13 +184,14 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
     // (a hint that is too small keeps every sequence in the few-rows kernel; one that is too large costs an idle launch)
     if (!(most > limit && S == 1 && max_q >= T && all > kFewRows)) {
         const int64_t rows_each = std::min<int64_t>(most, limit), tiles16 = tiles_of(16, rows_each);
-        const bool rows16 = rows_each <= 16 || (tiles16 * Hkv <= kCus && little(tiles16));
+        const bool rows16 = rows_each <= 16 || (tiles16 * Hkv <= kCus && (double)tiles16 * Hkv * keys < kSmall16);
         plan(rows16 ? 16 : 32, 1, limit, kWholeTilesFew, c.few, c.few_grid, c.few_bytes);
         c.few.waves = c.few.parts == 0 && c.few_grid > kCus ? kFewWaves : kManyWaves;
     }
     if (most > limit) plan(256, limit + 1, 0x7fffffff, kWholeTilesChunk, c.chunk, c.chunk_grid, c.chunk_bytes);
     // In key steps of about 1 us (few rows) and 2 us (chunks).  Equal pieces beside the line, chunks: 2048 rows x 4096 keys 62 us
-    // with and 74 without, 32 sequences of 128 rows x 4096 keys 177 and 191, where all units are busy anyway no difference; few rows: none.
+    // with and 74 without, 32 sequences of 128 rows x 4096 keys 177 and 191; no difference where all units are busy anyway, and
+    // none for few rows.
     c.few.min_steps = 8, c.few.piece_cost = 2, c.few.join_cost = 2, c.few.even = 0;
     c.chunk.min_steps = 4, c.chunk.piece_cost = 8, c.chunk.join_cost = 10, c.chunk.even = 1;
     return c;
