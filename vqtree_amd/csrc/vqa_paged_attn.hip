@@ -134,13 +134,15 @@ constexpr int kWholeSteps = 32;
 // Sequences of more rows than this go to the chunk kernel, which reads the keys once for 256 rows where the few-rows kernel
 // does for 32, at a higher rate of products, but starts and ends slower: few / chunk, 32 new tokens for 4 x 8 heads (128 rows):
 // 32 sequences of 4096 keys 221 / 192 us, 8 of 2000 to 8300 keys 101 / 75; 16 new tokens (64 rows), one sequence of 4096 or
-// 32768 keys 21 / 29, 38 / 58.  Calls with little to do stay in the few-rows kernel: tiles of 32 rows x key heads x keys, as far
-// as the host knows them, below kSmall.  128 rows, 8 sequences of 100 to 900 keys (0.2 M): 18 / 39; 256 rows x 4096 keys (0.3 M):
-// 26 / 38; 1024 rows x 1500 keys (0.4 M): 23 / 52; 512 rows, 8 sequences of 230 to 580 keys (0.6 M): 33 / 41; 2048 rows x 1500
-// keys (0.8 M): 32 / 53; 128 rows x 32768 keys (1.0 M): 51 / 60; 1024 rows, 8 sequences of 360 to 710 keys (1.5 M): 68 / 47; 256
-// rows x 32768 keys (2.1 M): 83 / 65.
+// 32768 keys 21 / 29, 38 / 58.  Calls with little to do stay in the few-rows kernel: tiles of 32 rows x key heads x (keys, as far
+// as the host knows them, and kTileKeys for the ends of a tile) below kSmall.  1024 rows x 1500 keys (0.5 M): 23 / 52; 256 rows,
+// 8 sequences of 160 to 510 keys, and 512 of 230 to 580 (0.6, 1.1 M): 21 / 43, 33 / 41; 20 to 230 rows of 21 sequences and 12
+// heads, window 77 (0.8 M): 32 / 52; 2048 rows x 1500 keys (1.0 M): 32 / 53; 128 rows x 32768 keys (1.1 M): 51 / 60; 2 sequences
+// of 7 x 1150 rows and 5 heads, window 51 (1.6 M): 54 / 52; 256 rows x 32768 keys (2.1 M): 83 / 65; 1024 rows, 8 sequences of 360
+// to 710 keys (2.5 M): 68 / 47; 26000 rows in 7 sequences and 5 heads, window 91 (2.8 M): 75 / 58.
 constexpr int kFewRows = 64;
-constexpr double kSmall = 5 << 18;
+constexpr double kSmall = 3 << 19;
+constexpr int kTileKeys = 512;
 
 // The few-rows kernel's tiles have 16 rows where that is all there are (one token / 16 sequences of it, 4 x 8 heads, 16 rows
 // against 32: 12.9 / 15.8, 193 / 223 us), and where a workgroup is left for each of them and little to read twice: 20 rows of 8
@@ -163,8 +165,7 @@ inline size_t o_bytes(const Plan& p, int Hkv, int D) { return round256((size_t)2
 inline size_t join_bytes(const Plan& p, int Hkv) { return round256((size_t)p.parts * Hkv * kJoinInts * 4); }
 inline size_t ml_bytes(const Plan& p, int Hkv) { return round256((size_t)2 * p.parts * Hkv * p.rows * 8); }
 
-// keys: most keys a row can see, as far as the caller's numbers tell
-inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t keys, bool e4m3) {
+inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int page, int width, int causal, int window, int max_q) {
     const int G = Hq / Hkv;
     Cut c{};
     const int64_t most = (int64_t)std::max(1, std::min(max_q, T)) * G;  // rows of a sequence
@@ -172,11 +173,16 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
     auto tiles_of = [&](int rows, int64_t rows_each) {  // at most, over all sequences
         return std::min(all / rows + seqs, seqs * ((rows_each + rows - 1) / rows));
     };
-    const int limit = most <= kFewRows || (double)tiles_of(32, most) * Hkv * keys < kSmall ? 0x7fffffff : kFewRows;
-    const bool short_keys = keys <= (int64_t)kWholeSteps * kKeyStep;
+    // most keys a tile can see, as far as the caller's numbers tell
+    auto keys_of = [&](int rows) {
+        const int64_t held = (int64_t)width * page;
+        return causal && window >= 0 ? std::min(held, (int64_t)window + (rows - 1) / G + 2 + kKeyStep) : held;
+    };
+    const int limit = most <= kFewRows || (double)tiles_of(32, most) * Hkv * (keys_of(32) + kTileKeys) < kSmall ? 0x7fffffff : kFewRows;
     auto plan = [&](int rows, int lo, int hi, int whole_from, Plan& p, int64_t& grid, size_t& bytes) {
         const int64_t tiles = tiles_of(rows, std::min<int64_t>(most, hi));
         p.rows = rows, p.lo = lo, p.hi = hi;
+        const bool short_keys = keys_of(rows) <= (int64_t)kWholeSteps * kKeyStep;
         p.parts = tiles * Hkv >= whole_from || short_keys ? 0 : std::max(1, kCus / Hkv);
         grid = (p.parts ? p.parts : tiles) * Hkv;
         bytes = o_bytes(p, Hkv, D) + ml_bytes(p, Hkv) + join_bytes(p, Hkv);
@@ -184,7 +190,7 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
     // (a hint that is too small keeps every sequence in the few-rows kernel; one that is too large costs an idle launch)
     if (!(most > limit && S == 1 && max_q >= T && all > kFewRows)) {
         const int64_t rows_each = std::min<int64_t>(most, limit), tiles16 = tiles_of(16, rows_each);
-        const bool rows16 = rows_each <= 16 || (tiles16 * Hkv <= kCus && (double)tiles16 * Hkv * keys < kSmall16);
+        const bool rows16 = rows_each <= 16 || (tiles16 * Hkv <= kCus && (double)tiles16 * Hkv * keys_of(16) < kSmall16);
         plan(rows16 ? 16 : 32, 1, limit, kWholeTilesFew, c.few, c.few_grid, c.few_bytes);
         c.few.waves = c.few.parts == 0 && c.few_grid > kCus ? kFewWaves : kManyWaves;
     }
@@ -195,11 +201,6 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int max_q, int64_t key
     c.few.min_steps = 8, c.few.piece_cost = 2, c.few.join_cost = 2, c.few.even = 0;
     c.chunk.min_steps = 4, c.chunk.piece_cost = 8, c.chunk.join_cost = 10, c.chunk.even = 1;
     return c;
-}
-
-inline int64_t most_keys(int width, int page, int causal, int window, int T, int max_q) {
-    const int64_t held = (int64_t)width * page;
-    return causal && window >= 0 ? std::min(held, (int64_t)window + std::max(1, std::min(max_q, T)) + kKeyStep) : held;
 }
 
 template <typename Tag>
@@ -251,7 +252,7 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
     a.window = window < 0 ? 1 << 30 : std::min(window, 1 << 30);
     a.scale_log2e = scale * kLog2e;
     if (S == 0 || T == 0) return VQA_OK;
-    Cut c = cut_call(T, S, Hq, Hkv, D, max_q, most_keys(width, page, causal, window, T, max_q), e4m3 != 0);
+    Cut c = cut_call(T, S, Hq, Hkv, D, page, width, causal, window, max_q);
     if (c.few_grid > 0x7fffffff || c.chunk_grid > 0x7fffffff) return VQA_ERR_BAD_SHAPE;
     const size_t bytes = c.few_bytes + c.chunk_bytes;
     if (bytes && ws == nullptr) return VQA_ERR_NULL_POINTER;
@@ -268,8 +269,7 @@ extern "C" {
 size_t vqa_paged_attn_workspace_bytes(int T, int S, int Hq, int Hkv, int D, int page, int width, int e4m3, int causal,
                                       int window, int max_q) {
     if (T < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || page < 1 || width < 1) return 0;
-    const vqa::paged::Cut c = vqa::paged::cut_call(
-        T, S, Hq, Hkv, D, max_q, vqa::paged::most_keys(width, page, causal, window, T, max_q), e4m3 != 0);
+    const vqa::paged::Cut c = vqa::paged::cut_call(T, S, Hq, Hkv, D, page, width, causal, window, max_q);
     return c.few_bytes + c.chunk_bytes;
 }
 

@@ -5,9 +5,9 @@
 // One sequence of 1000 keys is latency: 12.5 us -- 2 until the work is dealt out, 1 until the first tile is asked for, 4 for
 // four tiles per wave, 3 to join the waves.
 //
-// One workgroup of 8 waves, or 4 where there are enough tiles for two workgroups on a compute unit (the start and the end of one
-// under the loads of the other), works on one piece of a tile's keys at a time; its waves take consecutive parts of it and never wait for
-// each other until their results are joined at the end.  A wave walks 32-key tiles: the rows go HBM -> LDS directly
+// One workgroup of 8 waves, or 4 where there are enough tiles for two workgroups on a compute unit (the start and the end of
+// one under the loads of the other), works on one piece of a tile's keys at a time; its waves take consecutive parts of it and
+// never wait for each other until their results are joined at the end.  A wave walks 32-key tiles: the rows go HBM -> LDS directly
 // (global_load_lds_dwordx4, whole rows per instruction, no registers), S^T = K.Q^T and O^T = V^T.P^T run on
 // v_mfma_f32_16x16x32 -- the matrix pipe has room to spare at any memory rate, so a single query row goes through it too.
 //
