@@ -524,3 +524,74 @@ def test_a_run_of_steps(e4m3):
     last = q[new[0] - 1].view(1, H * G, 1, D)
     dense = attn_exact_decode(last, k[:1].repeat_interleave(G, 1), v[:1].repeat_interleave(G, 1))
     assert (dense[0, :, 0].float() - got[0][new[0] - 1].float()).abs().max() <= 2.0**-6
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# new rows fewer than the buffer has room for
+def poisoned_lse(rows, heads):
+    """Leaves a block of NaN where the allocator takes the next [rows, heads] fp32 tensor from."""
+    torch.full((rows, heads), math.nan, device=DEV)
+
+
+@both_widths
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("G", [1, 4])
+@pytest.mark.parametrize("n", [1, 5, 16, 40, 64, 65, 200])
+def test_one_sequence_in_a_longer_buffer(n, G, e4m3):
+    """The last chunk of a prompt fed through a buffer of fixed size: the sequence has the rows cu_q names, not the buffer's."""
+    T, Hkv, D = 256, 2, 64
+    c = Cache([n], [300], Hkv=Hkv, G=G, D=D, page=64, e4m3=e4m3, seed=30)
+    want = c.want()
+    q = torch.cat([c.q, torch.full((T - n, Hkv * G, D), math.nan, dtype=c.dtype)]).to(DEV)
+    for max_q in (None, T, 10**9, n):
+        out = torch.full((T, Hkv * G, D), 5.0, dtype=c.dtype, device=DEV)
+        poisoned_lse(T, Hkv * G)
+        got, lse = c.attend(q, out=out, return_lse=True, max_q_len=max_q)
+        compare((got[:n], lse[:n]), want, c)
+        assert (out[n:] == 5).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("width", [8, 1024])
+@pytest.mark.parametrize("cuts", [
+    ([0, 5], [0, 200], [0, 16], [0, 17], [0, 0], [0, 200], [0, 1]),
+    ([0, 1, 33, 200], [0, 70, 71, 71], [0, 0, 16, 200], [0, 17, 34, 50], [0, 200, 200, 200], [0, 1, 2, 3]),
+], ids=["one_sequence", "three_sequences"])
+def test_recorded_attention_replays_on_other_chunks(cuts, width, e4m3):
+    """Recorded once over a buffer of 200 rows, replayed on chunks of other lengths: sequences cross the 64 rows (16 tokens of
+    4 heads) that part the two kernels in both directions."""
+    T, H, G, D, page, S = 200, 2, 4, 64, 128, len(cuts[0]) - 1
+    g = torch.Generator().manual_seed(31)
+    c = Cache([1], [1], Hkv=H, G=G, D=D, page=page, e4m3=e4m3, seed=32, extra=S * 8)
+    table = torch.full((S, width), -1, dtype=torch.int32)
+    table[:, :8] = torch.randperm(c.k.shape[0], generator=g)[:S * 8].view(S, 8)
+    q = torch.randn(T, H * G, D, generator=g).to(c.dtype)
+    cu, lens = (torch.zeros(n, dtype=torch.int32, device=DEV) for n in (S + 1, S))
+    out = torch.zeros(T, H * G, D, dtype=c.dtype, device=DEV)
+    args = (q.to(DEV), c.k.to(DEV), c.v.to(DEV), table.to(DEV), cu, lens)
+    exps = c.exps(DEV)
+
+    def step():
+        return P.attn_paged(*args, **exps, return_lse=True, out=out)[1]
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lse = step()
+    for i, cut in enumerate(cuts):
+        print("cut", cut, flush=True)
+        new = [b - a for a, b in zip(cut, cut[1:])]
+        c.lens = [n + 50 + 211 * s + 97 * i for s, n in enumerate(new)]
+        cu.copy_(torch.tensor(cut, dtype=torch.int32))
+        lens.copy_(torch.tensor(c.lens, dtype=torch.int32))
+        out.fill_(5.0), lse.fill_(math.nan)
+        graph.replay()
+        n = cut[-1]
+        want = O.paged_attention(q[:n], c.k, c.v, table, torch.tensor(cut), torch.tensor(c.lens), **c.exps())
+        compare((out[:n], lse[:n]), want, c)
+        assert (out[n:] == 5).all()
+        replayed = out.clone()
+        out.fill_(5.0)
+        step()
+        assert torch.equal(replayed, out)

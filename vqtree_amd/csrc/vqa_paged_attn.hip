@@ -187,14 +187,17 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int page, int width, i
         grid = (p.parts ? p.parts : tiles) * Hkv;
         bytes = o_bytes(p, Hkv, D) + ml_bytes(p, Hkv) + join_bytes(p, Hkv);
     };
-    // (a hint that is too small keeps every sequence in the few-rows kernel; one that is too large costs an idle launch)
-    if (!(most > limit && S == 1 && max_q >= T && all > kFewRows)) {
+    // A hint that is too small keeps every sequence in the few-rows kernel; one that is too large costs an idle launch.  One
+    // sequence that may bring as many rows as the call has room for goes to the chunk kernel alone, however few it brings: how
+    // many there are only the device knows.
+    const bool chunk_alone = most > limit && S == 1 && max_q >= T && all > kFewRows;
+    if (!chunk_alone) {
         const int64_t rows_each = std::min<int64_t>(most, limit), tiles16 = tiles_of(16, rows_each);
         const bool rows16 = rows_each <= 16 || (tiles16 * Hkv <= kCus && (double)tiles16 * Hkv * keys_of(16) < kSmall16);
         plan(rows16 ? 16 : 32, 1, limit, kWholeTilesFew, c.few, c.few_grid, c.few_bytes);
         c.few.waves = c.few.parts == 0 && c.few_grid > kCus ? kFewWaves : kManyWaves;
     }
-    if (most > limit) plan(256, limit + 1, 0x7fffffff, kWholeTilesChunk, c.chunk, c.chunk_grid, c.chunk_bytes);
+    if (most > limit) plan(256, chunk_alone ? 1 : limit + 1, 0x7fffffff, kWholeTilesChunk, c.chunk, c.chunk_grid, c.chunk_bytes);
     // In key steps of about 1 us (few rows) and 2 us (chunks).  Equal pieces beside the line, chunks: 2048 rows x 4096 keys 62 us
     // with and 74 without, 32 sequences of 128 rows x 4096 keys 177 and 191; no difference where all units are busy anyway, and
     // none for few rows.
