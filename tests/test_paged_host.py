@@ -138,3 +138,24 @@ def test_c_entries_refuse_before_any_launch(lib):
     assert read(q=None) == -1 and read(S=1 << 17) == -2 and read(n=-1) == -2 and read(q=8) == -5 and read(n=0) == 0
     bad = _lib.strides_array(*([4] * 17))
     assert lib.vqa_paged_read_f16(16, 16, None, None, 16, 16, 16, 16, 2, 2, 5, 64, 16, 3, 2, 0, bad, None) == -5
+
+
+def test_numbers_given_as_tensors_are_read_at_every_call(lib, monkeypatch):
+    """What is kept of a call follows from values: a window, a hint or a number of rows held in a tensor counts as it is now."""
+    calls = []
+    monkeypatch.setattr(P, "_check_devices", lambda *a: None)
+    monkeypatch.setattr(P, "_launch", lambda fn, dev, *a: calls.append(a))
+    a = _call()
+    n, window, longest, scale = torch.tensor(30), torch.tensor(20), torch.tensor(4), torch.tensor(0.5)
+    for _ in range(2):
+        k, v = P.paged_read(a["k_pages"], a["v_pages"], a["block_table"], a["kv_lens"], n)
+        S, H, rows, D = calls[-1][8:12]
+        strides = list(calls[-1][-1])
+        assert (S, H, rows, D) == tuple(k.shape) == tuple(v.shape) == (2, 2, int(n), 64)
+        assert strides[11:14] == list(k.stride()[:3]) and strides[14:] == list(v.stride()[:3])
+        P.attn_paged(**a, window=window, max_q_len=longest, softmax_scale=scale)
+        causal, w, max_q, s = calls[-1][-4:]
+        assert (causal, w, max_q, s) == (1, int(window), int(longest), float(scale))
+        n.fill_(4), window.fill_(3), longest.fill_(1), scale.fill_(0.25)
+    with pytest.raises(TypeError):
+        P.paged_read(a["k_pages"], a["v_pages"], a["block_table"], a["kv_lens"], 4.0)

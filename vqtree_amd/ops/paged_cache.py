@@ -17,6 +17,7 @@ the other operators take.  Lengths and tables are read on the device when the ke
 graph replays on new ones.  Sequences of one call must not write to the same page (they may read the same one).
 """
 import math
+import operator
 
 import torch
 
@@ -28,7 +29,8 @@ E4M3 = torch.float8_e4m3fn
 
 # A generation step is a few microseconds of GPU work, so the host side counts.  What follows from shapes, strides, types and
 # options alone -- the checks, the strides array, the workspace's size -- is worked out once for each combination of them and
-# kept (_PLANS); a call then looks that up, checks the devices, and hands over the addresses.
+# kept (_PLANS); a call then looks that up, checks the devices, and hands over the addresses.  A key holds plain values only:
+# a number that comes as a tensor would be found again by its identity, whatever has become of its value.
 _PLANS = {}
 _MOST_PLANS = 4096
 
@@ -145,6 +147,7 @@ def _plan_write(k, v, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp
 def paged_read(k_pages, v_pages, block_table, kv_lens, n, *, k_exp=None, v_exp=None, dtype=None):
     """(k, v) [S,Hkv,n,D]: the first n rows of every sequence as plain tensors, zeros from kv_lens[s] on and on pages that
     are not there.  `dtype`: the element type of the result (8-bit pages: required; else the pages' own)."""
+    n = operator.index(n)
     key = ("r", k_pages.shape, k_pages.stride(), k_pages.dtype, v_pages.shape, v_pages.stride(), v_pages.dtype,
            block_table.shape, block_table.stride(), block_table.dtype, kv_lens.shape, kv_lens.stride(), kv_lens.dtype,
            _sig(k_exp), _sig(v_exp), n, dtype)
@@ -182,6 +185,13 @@ def attn_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, *, k_exp=None, v
     return_lse, the base-2 log-sum-exp [T,Hq] fp32: a state `merge_state_in_place` can combine.  A row that sees no key
     gets 0 and -inf; rows behind the last sequence are left as they are (`out`: the buffer to write to).
     `max_q_len`: the most new tokens any sequence has, where the caller knows it; it steers the choice of kernels only."""
+    causal = bool(causal)
+    if softmax_scale is not None:
+        softmax_scale = float(softmax_scale)
+    if window is not None:
+        window = int(window)
+    if max_q_len is not None:
+        max_q_len = int(max_q_len)
     key = ("a", q.shape, q.stride(), q.dtype, k_pages.shape, k_pages.stride(), k_pages.dtype, v_pages.shape,
            v_pages.stride(), v_pages.dtype, block_table.shape, block_table.stride(), block_table.dtype, cu_q.shape,
            cu_q.stride(), cu_q.dtype, kv_lens.shape, kv_lens.stride(), kv_lens.dtype, _sig(k_exp), _sig(v_exp), _sig(out),
@@ -222,9 +232,9 @@ def _plan_attn(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_exp, v_exp, so
     if T == 0 or S == 0 or q.stride(2) != 1:
         return None, 0, None
     lib = _lib.load()
-    max_q = T if max_q_len is None else max(0, min(int(max_q_len), T))
+    max_q = T if max_q_len is None else max(0, min(max_q_len, T))
     causal = 1 if causal else 0
-    window = -1 if window is None else min(int(window), (1 << 31) - 1)
+    window = -1 if window is None else min(window, (1 << 31) - 1)
     ws_bytes = lib.vqa_paged_attn_workspace_bytes(T, S, Hq, Hkv, D, page, width, e4m3, causal, window, max_q)
     out_strides = (Hq * D, D) if out is None else out.stride()[:2]
     strides = _lib.strides_array(*q.stride()[:2], *strides, *exp_strides, table_stride, *out_strides)
