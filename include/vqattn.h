@@ -10,7 +10,7 @@
  *     that need more than 64 KB (the count kernel at head dim 128, the pipelined prefill / window kernels, the paged
  *     attention) and the device address of that array.  Both belong to the device that owns the call's operands, which
  *     must be the calling thread's current device (VQA_ERR_BAD_ARGUMENT otherwise: the kernels would be launched
- *     elsewhere),
+ *     elsewhere; vqa_paged_write_* and vqa_paged_read_*, which need no set-up, ask the same at every call),
  *   - returns VQA_OK (0) or a negative vqa_status; it never throws or aborts.
  * Tensors are addressed as base + sum(index_i * stride_i) in ELEMENTS of their own type; the innermost
  * (head_dim / codebook index M) stride must be 1.  Head dims of the attention entry points: 64 and 128; vqa_local_attn_*,

@@ -1,5 +1,8 @@
 """Paged cache, CPU side: the 64-bit oracle against independent statements, and what the entry points refuse."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -159,3 +162,71 @@ def test_numbers_given_as_tensors_are_read_at_every_call(lib, monkeypatch):
         n.fill_(4), window.fill_(3), longest.fill_(1), scale.fill_(0.25)
     with pytest.raises(TypeError):
         P.paged_read(a["k_pages"], a["v_pages"], a["block_table"], a["kv_lens"], 4.0)
+
+
+# A HIP runtime of two devices that launches nothing: every pointer lies on `owner`.
+RUNTIME = """
+#include <string.h>
+typedef struct { int type, device; void *device_pointer, *host_pointer; int managed; unsigned flags; } attributes;
+typedef struct { unsigned x, y, z; } dim3_t;
+int current = 0, owner = 0, launches = 0;
+int hipGetDevice(int* d) { *d = current; return 0; }
+int hipPointerGetAttributes(attributes* a, const void* p) {
+    memset(a, 0, sizeof *a);
+    a->type = 2, a->device = owner, a->device_pointer = (void*)p;
+    return 0;
+}
+int hipFuncSetAttribute(const void* f, int a, int v) { return 0; }
+int hipGetLastError(void) { return 0; }
+int hipLaunchKernel(const void* f, dim3_t g, dim3_t b, void** args, size_t lds, void* stream) { ++launches; return 0; }
+int __hipPushCallConfiguration(dim3_t g, dim3_t b, size_t lds, void* stream) { return 0; }
+int __hipPopCallConfiguration(dim3_t* g, dim3_t* b, size_t* lds, void** stream) {
+    g->x = g->y = g->z = b->x = b->y = b->z = 1, *lds = 0, *stream = 0;
+    return 0;
+}
+"""
+
+TWO_DEVICES = """
+import ctypes, sys
+stub = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)  # (found before the runtime the library brings with it)
+sys.path.insert(0, sys.argv[2])
+from vqtree_amd import _lib
+lib = _lib.load()
+number = lambda name: ctypes.c_int.in_dll(stub, name)
+st = _lib.strides_array(*([128] * 17))
+
+def attn(T, S, Hkv, D, width):
+    need = lib.vqa_paged_attn_workspace_bytes(T, S, Hkv, Hkv, D, 16, width, 0, 1, -1, T)
+    return lib.vqa_paged_attn_bf16(16, 16, 16, None, None, 16, 16, 16, 16, None, 256, need, T, S, Hkv, Hkv, D, 16, 3, width,
+                                   0, st, 1, -1, T, 1.0, None)
+
+calls = {
+    "single token": lambda: attn(1, 1, 2, 128, 8),
+    "single tokens, narrow workgroups": lambda: attn(300, 300, 2, 128, 8),
+    "chunk": lambda: attn(512, 1, 2, 64, 16384),
+    "chunk, head dim 128": lambda: attn(512, 1, 2, 128, 16384),
+    "write": lambda: lib.vqa_paged_write_bf16(16, 16, 16, 16, None, None, 16, 16, 16, 4, 2, 2, 64, 16, 3, 2, 0, st, None),
+    "read": lambda: lib.vqa_paged_read_bf16(16, 16, None, None, 16, 16, 16, 16, 2, 2, 5, 64, 16, 3, 2, 0, st, None),
+}
+for turn in range(2):  # (the second time everything is set up on both devices)
+    for name, call in calls.items():
+        for device in (0, 1):
+            for owner in (0, 1):
+                number("current").value, number("owner").value, number("launches").value = device, owner, 0
+                rc, n = call(), number("launches").value
+                good = (rc == 0 and n > 0) if device == owner else (rc == -7 and n == 0)
+                if not good:
+                    print(name, "turn", turn, "device", device, "owner", owner, "status", rc, "launches", n)
+print("done")
+"""
+
+
+def test_operands_of_another_device_are_refused_at_every_call(tmp_path, lib):
+    source, stub = tmp_path / "runtime.c", tmp_path / "runtime.so"
+    source.write_text(RUNTIME)
+    subprocess.run(["gcc", "-shared", "-fPIC", "-w", "-include", "stddef.h", str(source), "-o", str(stub)], check=True)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(P.__file__)))
+    got = subprocess.run([sys.executable, "-c", TWO_DEVICES, str(stub), os.path.dirname(root)], capture_output=True, text=True,
+                         timeout=120)
+    assert got.returncode == 0, got.stderr
+    assert got.stdout == "done\n", got.stdout

@@ -434,15 +434,12 @@ __device__ __forceinline__ void for_each_piece(const AttnArgs& a, const Plan& p,
     }
 }
 
-// Kernels that use more than 64 KB of LDS need the limit raised once per device: the one that owns the operands.
+// Kernels that use more than 64 KB of LDS need the limit raised once per device: `dev`, the one that owns the operands.
 template <auto kKernel>
-int raise_lds(const void* operand, int bytes) {
+int raise_lds(int dev, int bytes) {
     static std::mutex mutex;
     static std::atomic<bool> raised[kMaxDevices];
-    int dev = 0;
-    if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < kMaxDevices && raised[dev].load(std::memory_order_acquire))
-        return VQA_OK;
-    if (int rc = device_of_pointer(operand, &dev)) return rc;
+    if (raised[dev].load(std::memory_order_acquire)) return VQA_OK;
     std::lock_guard<std::mutex> lock(mutex);
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
         hipSuccess) {
@@ -454,9 +451,9 @@ int raise_lds(const void* operand, int bytes) {
 }
 
 template <typename Tag>
-int launch_few(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream);
+int launch_few(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, int dev, hipStream_t stream);
 template <typename Tag>
-int launch_chunk(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream);
+int launch_chunk(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, int dev, hipStream_t stream);
 
 }  // namespace paged
 }  // namespace vqa

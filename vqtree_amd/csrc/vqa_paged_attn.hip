@@ -207,7 +207,7 @@ inline Cut cut_call(int T, int S, int Hq, int Hkv, int D, int page, int width, i
 }
 
 template <typename Tag>
-int run(const AttnArgs& a, Cut& c, void* ws, int D, bool e4m3, hipStream_t stream) {
+int run(const AttnArgs& a, Cut& c, void* ws, int D, bool e4m3, int dev, hipStream_t stream) {
     char* at = (char*)ws;
     for (Plan* p : {&c.few, &c.chunk}) {
         p->o = (float*)at;
@@ -218,9 +218,9 @@ int run(const AttnArgs& a, Cut& c, void* ws, int D, bool e4m3, hipStream_t strea
         at += join_bytes(*p, a.Hkv);
     }
     if (c.chunk.rows)
-        if (int rc = launch_chunk<Tag>(a, c.chunk, D, e4m3, c.chunk_grid, stream)) return rc;
+        if (int rc = launch_chunk<Tag>(a, c.chunk, D, e4m3, c.chunk_grid, dev, stream)) return rc;
     if (c.few.rows)
-        if (int rc = launch_few<Tag>(a, c.few, D, e4m3, c.few_grid, stream)) return rc;
+        if (int rc = launch_few<Tag>(a, c.few, D, e4m3, c.few_grid, dev, stream)) return rc;
     if (c.few.parts || c.chunk.parts) {
         const dim3 grid(c.chunk.parts ? 2 * kCus : kCus, 1, c.few.parts && c.chunk.parts ? 2 : 1);
         if (D == 128)
@@ -261,7 +261,9 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
     if (bytes && ws == nullptr) return VQA_ERR_NULL_POINTER;
     if (reinterpret_cast<uintptr_t>(ws) % 256) return VQA_ERR_MISALIGNED;
     if (ws_bytes < bytes) return VQA_ERR_WORKSPACE_TOO_SMALL;
-    return run<Tag>(a, c, ws, D, e4m3 != 0, stream);
+    int dev = 0;
+    if (int rc = device_of_pointer(q, &dev)) return rc;
+    return run<Tag>(a, c, ws, D, e4m3 != 0, dev, stream);
 }
 
 }  // namespace paged

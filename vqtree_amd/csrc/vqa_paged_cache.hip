@@ -188,6 +188,8 @@ int write(const void* k, const void* v, void* k_pages, void* v_pages, uint8_t* k
     const int rows = kWriteWaves * 64 / (D / 16);
     const int64_t blocks = (int64_t)((T + rows - 1) / rows) * H;
     if (blocks > 0x7fffffff) return VQA_ERR_BAD_SHAPE;
+    int dev = 0;
+    if (int rc = device_of_pointer(k, &dev)) return rc;
     const dim3 grid((unsigned)blocks);
     if (D == 128)
         write_kernel<Tag, 128><<<grid, kWriteWaves * 64, 0, stream>>>(a);
@@ -210,6 +212,8 @@ int read(const void* k_pages, const void* v_pages, const uint8_t* k_exp, const u
     if (!aligned16(k) || !aligned16(v) || (st[11] | st[12] | st[13] | st[14] | st[15] | st[16]) % 8)
         return VQA_ERR_MISALIGNED;
     if (S == 0 || n == 0) return VQA_OK;
+    int dev = 0;
+    if (int rc = device_of_pointer(k, &dev)) return rc;
     const int rows = kReadWaves * kReadRounds * 64 / (D / 8);
     const dim3 grid((n + rows - 1) / rows, H, S);
     if (D == 128 && e4m3)

@@ -514,12 +514,12 @@ __global__ __launch_bounds__(kWaves * 64, 1) void chunk_kernel(AttnArgs a, Plan 
 }
 
 template <typename Tag, int D, bool kE4m3>
-int launch(const AttnArgs& a, const Plan& p, int64_t grid, hipStream_t stream) {
+int launch(const AttnArgs& a, const Plan& p, int64_t grid, int dev, hipStream_t stream) {
     constexpr int tiles = 4 * Geom<D>::kTileBytes + (kE4m3 ? 2 * kWaves * Raw<D>::kBytes : 0);
     constexpr int stage = kWaves * flash2::Pipe<Tag, D, kWaves, true>::kStoreBytes;
     constexpr int bytes = tiles > stage ? tiles : stage;
     if (bytes > 64 * 1024)
-        if (int rc = raise_lds<chunk_kernel<Tag, D, kE4m3>>(a.q, bytes)) return rc;
+        if (int rc = raise_lds<chunk_kernel<Tag, D, kE4m3>>(dev, bytes)) return rc;
     chunk_kernel<Tag, D, kE4m3><<<dim3((unsigned)grid), kWaves * 64, bytes, stream>>>(a, p);
     return launch_status();
 }
@@ -527,13 +527,13 @@ int launch(const AttnArgs& a, const Plan& p, int64_t grid, hipStream_t stream) {
 }  // namespace chunk
 
 template <typename Tag>
-int launch_chunk(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream) {
+int launch_chunk(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, int dev, hipStream_t stream) {
     if (D == 128)
-        return e4m3 ? chunk::launch<Tag, 128, true>(a, p, grid, stream) : chunk::launch<Tag, 128, false>(a, p, grid, stream);
-    return e4m3 ? chunk::launch<Tag, 64, true>(a, p, grid, stream) : chunk::launch<Tag, 64, false>(a, p, grid, stream);
+        return e4m3 ? chunk::launch<Tag, 128, true>(a, p, grid, dev, stream) : chunk::launch<Tag, 128, false>(a, p, grid, dev, stream);
+    return e4m3 ? chunk::launch<Tag, 64, true>(a, p, grid, dev, stream) : chunk::launch<Tag, 64, false>(a, p, grid, dev, stream);
 }
-template int launch_chunk<bf16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);
-template int launch_chunk<f16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);
+template int launch_chunk<bf16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, int, hipStream_t);
+template int launch_chunk<f16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, int, hipStream_t);
 
 }  // namespace paged
 }  // namespace vqa

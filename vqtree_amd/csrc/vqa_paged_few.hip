@@ -522,32 +522,32 @@ constexpr int lds_bytes() {
 }
 
 template <typename Tag, int D, bool kE4m3, int NB, int kWaves>
-int launch(const AttnArgs& a, const Plan& p, int64_t grid, hipStream_t stream) {
+int launch(const AttnArgs& a, const Plan& p, int64_t grid, int dev, hipStream_t stream) {
     constexpr int bytes = lds_bytes<D, kE4m3, NB, kWaves>();
     if (bytes > 64 * 1024) {
-        if (int rc = raise_lds<few_kernel<Tag, D, kE4m3, NB, kWaves>>(a.q, bytes)) return rc;
+        if (int rc = raise_lds<few_kernel<Tag, D, kE4m3, NB, kWaves>>(dev, bytes)) return rc;
     }
     few_kernel<Tag, D, kE4m3, NB, kWaves><<<dim3((unsigned)grid), kWaves * 64, bytes, stream>>>(a, p);
     return launch_status();
 }
 
 template <typename Tag, int D, bool kE4m3>
-int launch(const AttnArgs& a, const Plan& p, int64_t grid, hipStream_t stream) {
+int launch(const AttnArgs& a, const Plan& p, int64_t grid, int dev, hipStream_t stream) {
     if (p.waves == 4)
-        return p.rows == 32 ? launch<Tag, D, kE4m3, 2, 4>(a, p, grid, stream) : launch<Tag, D, kE4m3, 1, 4>(a, p, grid, stream);
-    return p.rows == 32 ? launch<Tag, D, kE4m3, 2, 8>(a, p, grid, stream) : launch<Tag, D, kE4m3, 1, 8>(a, p, grid, stream);
+        return p.rows == 32 ? launch<Tag, D, kE4m3, 2, 4>(a, p, grid, dev, stream) : launch<Tag, D, kE4m3, 1, 4>(a, p, grid, dev, stream);
+    return p.rows == 32 ? launch<Tag, D, kE4m3, 2, 8>(a, p, grid, dev, stream) : launch<Tag, D, kE4m3, 1, 8>(a, p, grid, dev, stream);
 }
 
 }  // namespace few
 
 template <typename Tag>
-int launch_few(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, hipStream_t stream) {
+int launch_few(const AttnArgs& a, const Plan& p, int D, bool e4m3, int64_t grid, int dev, hipStream_t stream) {
     if (D == 128)
-        return e4m3 ? few::launch<Tag, 128, true>(a, p, grid, stream) : few::launch<Tag, 128, false>(a, p, grid, stream);
-    return e4m3 ? few::launch<Tag, 64, true>(a, p, grid, stream) : few::launch<Tag, 64, false>(a, p, grid, stream);
+        return e4m3 ? few::launch<Tag, 128, true>(a, p, grid, dev, stream) : few::launch<Tag, 128, false>(a, p, grid, dev, stream);
+    return e4m3 ? few::launch<Tag, 64, true>(a, p, grid, dev, stream) : few::launch<Tag, 64, false>(a, p, grid, dev, stream);
 }
-template int launch_few<bf16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);
-template int launch_few<f16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, hipStream_t);
+template int launch_few<bf16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, int, hipStream_t);
+template int launch_few<f16_tag>(const AttnArgs&, const Plan&, int, bool, int64_t, int, hipStream_t);
 
 }  // namespace paged
 }  // namespace vqa
