@@ -595,3 +595,26 @@ def test_recorded_attention_replays_on_other_chunks(cuts, width, e4m3):
         out.fill_(5.0)
         step()
         assert torch.equal(replayed, out)
+
+
+@both_widths
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new", [[1, 2], [90, 3]])
+def test_lengths_up_to_the_largest_int(new, e4m3):
+    """More keys than any table has room for: the rows stand behind them all and, without a window, see them all; with one they
+    see what it leaves of them."""
+    c = Cache(new, [300, 30], D=64, page=128, G=2, e4m3=e4m3, seed=33)
+    for length in (2**30 + 500, 2**31 - 1):
+        c.kv_lens[0] = length
+        kept, c.lens = c.lens, [512, c.lens[1]]  # (the sums run over the keys the table holds)
+        got = c.attend(return_lse=True)
+        whole = c.want()
+        compare(got, whole, c)
+        compare(c.attend(return_lse=True, causal=False), c.want(causal=False), c)
+        n = new[0]
+        for window in (2**31 - 2, length - 200, 100):
+            out, lse = c.attend(return_lse=True, window=window)
+            compare((out, lse), c.want(window=window), c)
+            if window == 100:
+                assert (out[:n] == 0).all() and (lse[:n] == -math.inf).all()
+        c.lens = kept

@@ -23,7 +23,7 @@ struct AttnArgs {
     int64_t o_st, o_sh;
     float* lse;  // [T, Hq] contiguous, nullable
     int Hq, Hkv, G;
-    int causal, window;  // window: a number no distance reaches where there is none
+    int causal, window;  // window: the largest int, which no distance reaches, where there is none
     float scale_log2e;
 };
 
@@ -34,7 +34,8 @@ struct Range {
 __device__ __forceinline__ Range visible(const AttnArgs& a, const Seq& s, int t) {
     if (!a.causal) return {0, s.keys};
     const int i = s.len - s.n + t;
-    return {max(0, i - a.window), min(s.keys, i + 1)};
+    // (i may be negative, so i - window is formed where it is positive only)
+    return {i > a.window ? i - a.window : 0, min(s.keys, i + 1)};
 }
 
 // Unnormalised attention of ONE row over keys [lo, hi), by one wave in fp32: the definition, key by key.  A lane scores one

@@ -252,7 +252,7 @@ int attn(const void* q, const void* k_pages, const void* v_pages, const uint8_t*
     a.lse = lse;
     a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
     a.causal = causal != 0;
-    a.window = window < 0 ? 1 << 30 : std::min(window, 1 << 30);
+    a.window = window < 0 ? 0x7fffffff : window;
     a.scale_log2e = scale * kLog2e;
     if (S == 0 || T == 0) return VQA_OK;
     Cut c = cut_call(T, S, Hq, Hkv, D, page, width, causal, window, max_q);
