@@ -513,8 +513,8 @@ int vqa_count_step_f16(const void* q, const void* rope_cos, const void* rope_sin
  * brought into range there: a recorded call can be replayed on new lengths and tables.
  *
  * Storage (e4m3 = 0): the element type.  e4m3 = 1: one byte per element plus one byte per row, value =
- * e4m3 * 2^(byte - 127); the byte names the smallest power of two that brings the row into +-448.  Pages [.., page, D]
- * bytes, exponents k_exp / v_exp [n_pages, H, page], unit stride along the page.  Magnitudes beyond 1.875 * 2^15 (f16) or
+ * e4m3 * 2^(byte - 127); the byte names the smallest power of two that brings the row into +-448.  The write leaves bytes
+ * 1 .. 247; byte 0 counts as 1, and with one above 247 values may pass what the element type holds.  Pages [.., page, D] bytes, exponents k_exp / v_exp [n_pages, H, page], unit stride along the page.  Magnitudes beyond 1.875 * 2^15 (f16) or
  * 1.875 * 2^127 (bf16), infinities among them, are stored as that; NaN stays NaN.
  *
  * vqa_paged_write: rows k, v [T,H,D] of the new tokens into their places (no two sequences of a call may write to the

@@ -618,3 +618,20 @@ def test_lengths_up_to_the_largest_int(new, e4m3):
             if window == 100:
                 assert (out[:n] == 0).all() and (lse[:n] == -math.inf).all()
         c.lens = kept
+
+
+@both_widths
+@pytest.mark.parametrize("new", [[1], [20], [90]])
+def test_exponent_byte_0_counts_as_1(new):
+    """In every kernel and for keys and values alike: byte 0, which the write never leaves, is 2^-126 as byte 1 is."""
+    c = Cache(new, [200], D=64, page=16, G=2, e4m3=True, seed=34)
+    got = []
+    for low in (0, 1):
+        c.k_exp[:], c.v_exp[:] = 118, 1
+        c.v_exp[:, :, ::3], c.k_exp[:, :, 1::5] = low, low
+        out, lse = c.attend(return_lse=True)
+        k, v = P.paged_read(c.k.to(DEV), c.v.to(DEV), c.table.to(DEV), c.kv_lens.to(DEV), c.lens[0], dtype=c.dtype, **c.exps(DEV))
+        got.append((out, lse, k, v))
+    assert (got[0][0] != 0).any() and torch.isfinite(got[0][0]).all()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)

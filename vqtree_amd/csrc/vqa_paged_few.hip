@@ -360,7 +360,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(AttnArgs a, Plan p)
                     pr[e] = fast_exp2(__builtin_fmaf(s[b][e >> 2][e & 3], a.scale_log2e, -ref));
                     l[b] += pr[e];
                     if constexpr (kE4m3)
-                        pr[e] = __builtin_ldexpf(pr[e], (int)((vexp[e >> 2] >> (8 * (e & 3))) & 0xffu) - 127);
+                        pr[e] = __builtin_ldexpf(pr[e], max((int)((vexp[e >> 2] >> (8 * (e & 3))) & 0xffu), 1) - 127);
                 }
                 const u32x4_t pk = {Elem<PTag>::pack2(pr[0], pr[1]), Elem<PTag>::pack2(pr[2], pr[3]),
                                     Elem<PTag>::pack2(pr[4], pr[5]), Elem<PTag>::pack2(pr[6], pr[7])};

@@ -5,7 +5,7 @@ second chunk of a prompt ("Only support prefilling or generation", ops/attn_vq.p
 pages that sequences of any length share:
 
     k_pages, v_pages [pages, Hkv, page, D]   q's dtype, or torch.float8_e4m3fn with
-    k_exp, v_exp     [pages, Hkv, page]      uint8: value = e4m3 * 2^(byte - 127), one byte per row
+    k_exp, v_exp     [pages, Hkv, page]      uint8: value = e4m3 * 2^(byte - 127), one byte per row (0 counts as 1)
     block_table      [S, width] int32        the pages of each sequence, in order; -1 (or any number that is no page)
                                              where there is none
     kv_lens          [S] int32               keys of each sequence, new ones included
