@@ -635,3 +635,41 @@ def test_exponent_byte_0_counts_as_1(new):
     assert (got[0][0] != 0).any() and torch.isfinite(got[0][0]).all()
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@both_widths
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new,past,Hkv,G", [
+    ([1, 3], [400, 70], 1, 40), ([9], [300], 1, 130), ([1], [200], 1, 600), ([2, 1], [500, 33], 300, 1), ([66], [200], 300, 1),
+    ([1] * 300, [(37 * i) % 500 for i in range(300)], 1, 2), ([5, 0, 20] * 90, [(53 * i) % 300 for i in range(270)], 2, 4),
+], ids=["g40", "g130", "g600", "300_heads", "300_heads_chunk", "300_sequences", "270_sequences"])
+def test_many_heads_and_many_sequences(new, past, Hkv, G, e4m3):
+    """Groups of heads larger than a tile, more key heads than compute units, more sequences than a few waves hold."""
+    c = Cache(new, past, Hkv=Hkv, G=G, D=64, page=32, e4m3=e4m3, seed=35)
+    got = c.attend(return_lse=True)
+    compare(got, c.want(), c)
+
+
+@both_widths
+@pytest.mark.parametrize("new", [[1, 4], [90, 1]])
+def test_states_of_two_caches_merge(new):
+    """Attention over the first keys and over the rest, joined by merge_state_in_place, is attention over all of them.  Each of
+    the two states is within compare()'s tolerance of its part, the parts' weights add up to one, and the result is rounded once
+    more: 3 roundings instead of 2 (eps * A each); the weights follow the log-sum-exps, whose errors move a weight by ln 2 times
+    that, twice."""
+    from vqtree_amd.ops.triton_fused_vq_attn import merge_state_in_place
+
+    c = Cache(new, [300, 150], D=128, page=16, G=2, seed=36)
+    cut = 6  # pages; the second sequence's rows stand behind them too
+    args = (c.q.to(DEV), c.k.to(DEV), c.v.to(DEV))
+    cu = c.cu.to(DEV)
+    first = torch.full((2,), cut * 16, dtype=torch.int32, device=DEV)
+    a, sa = P.attn_paged(*args, c.table[:, :cut].to(DEV), cu, first, causal=False, return_lse=True)
+    b, sb = P.attn_paged(*args, c.table[:, cut:].contiguous().to(DEV), cu, c.kv_lens.to(DEV) - cut * 16, return_lse=True)
+    merge_state_in_place(a, sa, b, sb)
+    w_out, w_lse, A, Z = c.want()
+    eps, N = torch.finfo(c.dtype).eps / 2, max(c.lens)
+    lse_tol = ((c.D + 2) * Z + 2 * (N + 64) + 16) * 1.4427 * U + 8 * U * w_lse.abs()
+    tol = (3 * eps + (2 * (c.D + 2) * Z[..., None] + 2 * (N + 64) + 16) * U + 2 * 0.6932 * lse_tol[..., None]) * A
+    assert ((a.double().cpu() - w_out).abs() <= tol).all()
+    assert ((sa.double().cpu() - w_lse).abs() <= lse_tol).all()
