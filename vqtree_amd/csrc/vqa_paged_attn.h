@@ -34,8 +34,8 @@ struct Range {
 __device__ __forceinline__ Range visible(const AttnArgs& a, const Seq& s, int t) {
     if (!a.causal) return {0, s.keys};
     const int i = s.len - s.n + t;
-    // (i may be negative, so i - window is formed where it is positive only)
-    return {i > a.window ? i - a.window : 0, min(s.keys, i + 1)};
+    // (max(0, i - window) without overflow, i may be negative)
+    return {i - min(i, a.window), min(s.keys, i + 1)};
 }
 
 // Unnormalised attention of ONE row over keys [lo, hi), by one wave in fp32: the definition, key by key.  A lane scores one
