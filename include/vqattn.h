@@ -514,11 +514,12 @@ int vqa_count_step_f16(const void* q, const void* rope_cos, const void* rope_sin
  *
  * Storage (e4m3 = 0): the element type.  e4m3 = 1: one byte per element plus one byte per row, value =
  * e4m3 * 2^(byte - 127); the byte names the smallest power of two that brings the row into +-448.  The write leaves bytes
- * 1 .. 247; byte 0 counts as 1, and with one above 247 values may pass what the element type holds.  Pages [.., page, D] bytes, exponents k_exp / v_exp [n_pages, H, page], unit stride along the page.  Magnitudes beyond 1.875 * 2^15 (f16) or
+ * 1 .. 247; byte 0 counts as 1, and with one above 247 values may pass what the element type holds.  Pages [.., page, D]
+ * bytes, exponents k_exp / v_exp [n_pages, H, page], unit stride along the page.  Magnitudes beyond 1.875 * 2^15 (f16) or
  * 1.875 * 2^127 (bf16), infinities among them, are stored as that; NaN stays NaN.
  *
  * vqa_paged_write: rows k, v [T,H,D] of the new tokens into their places (no two sequences of a call may write to the
- *   same page).  strides[0..14] = k(t,h) v(t,h) k_pages(p,h,n) v_pages(p,h,n) k_exp(p,h) v_exp(p,h) table(s).
+ *   same page, and no sequence to one page through two entries of its table).  strides[0..14] = k(t,h) v(t,h) k_pages(p,h,n) v_pages(p,h,n) k_exp(p,h) v_exp(p,h) table(s).
  * vqa_paged_read: rows 0 .. n - 1 of every sequence as plain tensors k, v [S,H,n,D], zeros from kv_lens[s] on.
  *   strides[0..16] = k_pages(p,h,n) v_pages(p,h,n) k_exp(p,h) v_exp(p,h) table(s) k(s,h,n) v(s,h,n).  S <= 65535.
  * vqa_paged_attn: q [T,Hq,D] of the new tokens (Hq a multiple of Hkv; query head h reads key head h / (Hq / Hkv)) over

@@ -5,7 +5,7 @@
 // [pages, Hkv, page, D].  A table entry outside [0, pages) is a page that is not there: nothing is written to it, its rows
 // read as zero and its keys are hidden.  Rows come in the element type, or as e4m3 with one byte per row that holds a power of
 // two (value = e4m3 * 2^(byte - 127)): a power of two costs the values nothing -- e4m3 has four significant bits wherever a
-// row's largest magnitude lies -- and gfx950 converts with such a factor in the same instruction
+// row's largest magnitude lies, for that and for everything down to 2^-14 of it (below, its steps stay the same) -- and gfx950 converts with such a factor in the same instruction
 // (v_cvt_scalef32_pk_*_fp8), so what the attention multiplies is the stored value exactly, without a scale in the scores.
 #pragma once
 
@@ -61,8 +61,6 @@ __device__ __forceinline__ uint8_t* exp_of(const Pool& pool, const Seqs& g, int 
 __device__ __forceinline__ float factor_of(int byte) {
     return __builtin_bit_cast(float, (uint32_t)max(byte, 1) << 23);
 }
-
-typedef short s16x2_t __attribute__((ext_vector_type(2)));
 
 // four e4m3 values times a power of two, as two packed pairs of the element type: exact in bf16 (4 significant bits); in f16
 // exact down to its subnormal numbers, where the last place is rounded

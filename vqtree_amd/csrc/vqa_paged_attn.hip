@@ -135,7 +135,7 @@ constexpr int kWholeSteps = 32;
 // does for 32, at a higher rate of products, but starts and ends slower: few / chunk, 32 new tokens for 4 x 8 heads (128 rows):
 // 32 sequences of 4096 keys 221 / 192 us, 8 of 2000 to 8300 keys 101 / 75; 16 new tokens (64 rows), one sequence of 4096 or
 // 32768 keys 21 / 29, 38 / 58.  Calls with little to do stay in the few-rows kernel: tiles of 32 rows x key heads x (keys, as far
-// as the host knows them, and kTileKeys for the ends of a tile) below kSmall.  1024 rows x 1500 keys (0.5 M): 23 / 52; 256 rows,
+// as the host knows them -- what the table has room for, or the window -- and kTileKeys for the ends of a tile) below kSmall.  1024 rows x 1500 keys (0.5 M): 23 / 52; 256 rows,
 // 8 sequences of 160 to 510 keys, and 512 of 230 to 580 (0.6, 1.1 M): 21 / 43, 33 / 41; 20 to 230 rows of 21 sequences and 12
 // heads, window 77 (0.8 M): 32 / 52; 2048 rows x 1500 keys (1.0 M): 32 / 53; 128 rows x 32768 keys (1.1 M): 51 / 60; 2 sequences
 // of 7 x 1150 rows and 5 heads, window 51 (1.6 M): 54 / 52; 256 rows x 32768 keys (2.1 M): 83 / 65; 1024 rows, 8 sequences of 360

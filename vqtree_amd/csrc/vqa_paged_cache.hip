@@ -4,9 +4,10 @@
 //   Writing, a lane holds 16 elements of a row (8 lanes a row at head dim 128): with 8, which makes every load one contiguous
 // kilobyte, the quantiser's instructions per byte cost more than the loads gain (53 against 43 us for 8192 rows of 32 heads, keys
 // and values, in a loop over one input).  Workgroups go over the heads first (43 -> 40 us), stores past the caches (47 -> 44 us
-// in a loop over several inputs: 4.6 TB/s).
+// in a loop over several inputs: 4.6 TB/s).  16-bit pages: 56 us for 268 MB, 4.8 TB/s.
 //   Reading, a lane holds 8 elements, so that a wave stores contiguous kilobytes, and past the caches: 756 MB in 134 us,
-// 5.6 TB/s (in a loop over one input 105 us; 149 with ordinary stores, 214 with 16 elements per lane).
+// 5.6 TB/s (in a loop over one input 105 us; 149 with ordinary stores, 214 with 16 elements per lane).  16-bit pages:
+// 971 MB in 167 us, 5.8 TB/s.
 //
 // 8-bit rows.  The factor of a row is the smallest power of two 2^e with max |x| <= 448 * 2^e, 448 being the largest e4m3
 // number, so nothing saturates; the quotient is exact in fp32 and is rounded once, to the nearest e4m3 number (ties to even).

@@ -1,8 +1,8 @@
 // Many rows: chunks of prompts (vqa_paged_attn_*), on the software-pipelined core of vqa_flash2.h.  Bound by the issue of the
 // core's instructions beside its matrix products.  Measured, 2048 new tokens behind 8192, 32 query and 8 key heads, head dim
-// 128, 16 bits: 281 us a call among others, 1.10 PFLOP/s (a large library product: 1.35), matrix pipe 52 % busy; over an e4m3
-// cache 17 % more.  A workgroup takes 11 us until its first products and 5 to store its rows, 1.6 us per 64 keys between
-// (e4m3 2.0), so short pieces pay for their ends.
+// 128, 16 bits: 281 - 293 us a call among others, 1.06 - 1.10 PFLOP/s (a large library product: 1.35), matrix pipe 52 % busy;
+// over an e4m3 cache 17 % more.  A workgroup takes 10 us until its first products and 7 to store its rows, 1.7 us per 64 keys
+// between (e4m3: 12, 12 and 2.1), so short pieces pay for their ends.
 //
 // One workgroup of 4 waves owns a tile of 256 rows (grouped query heads and tokens together, so a chunk of 64 tokens with
 // 4 query heads per key head fills one) and walks 64-key tiles of the piece it was given; a wave brings 16 rows of each

@@ -2,7 +2,7 @@
 // row of a (sequence, key head) is read once for all rows of a tile, 16 * NB of them (grouped query heads and new tokens
 // together).  Measured (kernel time): 16 sequences, 260 000 keys together, 32 query and 8 key heads, head dim 128: 185 us for
 // 1.19 GB of 16-bit rows, 6.4 TB/s (reads alone reach about 7); 65 536 keys of 32 heads in e4m3: 92 us for 0.54 GB, 5.9 TB/s.
-// One sequence of 1000 keys is latency: 12.5 us -- 2 until the work is dealt out, 1 until the first tile is asked for, 4 for
+// One sequence of 1000 keys is latency: 13 us -- 2 until the work is dealt out, 1 until the first tile is asked for, 4 for
 // four tiles per wave, 3 to join the waves.
 //
 // One workgroup of 8 waves, or 4 where there are enough tiles for two workgroups on a compute unit (the start and the end of
@@ -22,7 +22,8 @@
 // then holds 8 keys of one d.
 //
 // Where the P.V product is in bf16, a probability is split into two bf16 numbers (16 bits together): the matrix pipe has the
-// time, and the output's error against 64 bits falls from 1.4 times that of its own rounding to 1.0 times.
+// time, and the output's error against 64 bits falls from 1.4 times that of its own rounding to 1.0 times.  In f16 (16-bit
+// pages) a probability has 11 bits as it is, and the error is 1.1 to 1.4 times that of the rounding.
 #include "vqa_flash2.h"
 #include "vqa_paged_attn.h"
 

@@ -14,7 +14,8 @@ pages that sequences of any length share:
 A step is `paged_write(k, v, ...)` and then `attn_paged(q, ...)` with the same table, `cu_q` and `kv_lens`, whether it
 brings one token per sequence, chunks of prompts, or both.  `paged_read` gives the cache back as the plain tensors that
 the other operators take.  Lengths and tables are read on the device when the kernels run: a step recorded into a HIP
-graph replays on new ones.  Sequences of one call must not write to the same page (they may read the same one).
+graph replays on new ones.  Sequences of one call must not write to the same page (they may read the same one), nor
+one sequence to a page that its table names twice.
 """
 import math
 import operator
@@ -184,7 +185,8 @@ def attn_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, *, k_exp=None, v
     multiple of the pages' heads; query head h reads key head h // (Hq // Hkv).  Returns out [T,Hq,D] (q's dtype) and, with
     return_lse, the base-2 log-sum-exp [T,Hq] fp32: a state `merge_state_in_place` can combine.  A row that sees no key
     gets 0 and -inf; rows behind the last sequence are left as they are (`out`: the buffer to write to).
-    `max_q_len`: the most new tokens any sequence has, where the caller knows it; it steers the choice of kernels only."""
+    `max_q_len`: the most new tokens any sequence has, where the caller knows it; it steers the choice of kernels only.
+    For the number of keys that choice goes by what block_table has room for."""
     causal = bool(causal)
     if softmax_scale is not None:
         softmax_scale = float(softmax_scale)
